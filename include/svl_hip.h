@@ -612,6 +612,132 @@ svl_status svl_vector_rank_device(svl_vector_index *index, const float *d_querie
                                   int64_t offset, int64_t limit, int64_t *out_index,
                                   double *out_score, int64_t *out_count, void *stream);
 
+/* ---- packed documents over several axes -------------------------------------- */
+/* Three operators for batches of documents packed back to back, in the form
+ * that encoders of images, video and long text take them: positions over
+ * (time, height, width), the rotation of queries and keys by them, and
+ * attention with masks, a score cap and a distance bias. The reference has no
+ * counterpart: its rotation takes one axis (kernels.rs:1014-1035) or the two
+ * of a picture (vision.rs), its attention one row with a symmetric window
+ * (kernels.rs:1037-1135).
+ *
+ * A plan holds what belongs to a batch and not to its numbers (lengths, masks,
+ * work items) in HBM; it is made once per batch and shared by the layers. The
+ * operators check their arguments on the host, enqueue on `stream` (NULL = the
+ * null stream) and return without waiting; nothing is allocated, read back or
+ * kept between calls, so calls can be recorded into HIP graphs, and several
+ * may run at once on the same plan, each with a workspace of its own. A plan
+ * outlives the work and the graphs that use it; making or destroying one waits
+ * for the device and is not recorded. Non-finite values pass through (no
+ * INTERNAL status as from the kernel seam, which would take a wait per call).
+ * A null pointer, a negative size or a shape that contradicts another ->
+ * USAGE, a size above a cap -> LIMIT, a type or head dim that no kernel takes
+ * -> UNSUPPORTED. */
+
+typedef struct svl_position_plan svl_position_plan;
+
+/* A run of text (frames tokens; rows, cols and step are not read) or a grid of
+ * frames x rows x cols tokens, row-major, of document `document` (ids do not
+ * decrease; a change starts a new document). A segment of no tokens adds
+ * nothing. */
+typedef enum { SVL_SEGMENT_TEXT = 0, SVL_SEGMENT_GRID = 1 } svl_segment_kind;
+typedef struct {
+    int64_t document;
+    int32_t kind;
+    int32_t frames, rows, cols;
+    int32_t step; /* positions from one frame to the next, at least 1 */
+} svl_segment;
+
+/* Positions start at 0 in each document. A text run at p takes
+ * (p + i, p + i, p + i) and moves p by its length; a grid at p takes
+ * (p + step * frame, p + row, p + col) and moves p past its largest extent,
+ * max(step * (frames - 1) + 1, rows, cols). At most 2^31 - 1 tokens, positions
+ * below 2^31 -> LIMIT. */
+svl_status svl_position_plan_create(svl_ctx *ctx, const svl_segment *segments, int64_t n,
+                                    svl_position_plan **out);
+svl_status svl_position_plan_destroy(svl_position_plan *plan);
+int64_t svl_position_plan_tokens(const svl_position_plan *plan);
+/* d_positions [tokens, 3] (time, height, width) of every token, in order, on
+ * the plan's device. */
+svl_status svl_axis_positions(const svl_position_plan *plan, int32_t *d_positions, void *stream);
+
+/* Which two columns of a head pair j = 0 .. pairs - 1 rotates: (j, j + pairs);
+ * (2 j, 2 j + 1); or, each run of pairs of one axis in a block of its own (as
+ * the vision tower's heads hold them), first + (i, i + run) for pair i of the
+ * run that starts at column first. */
+typedef enum { SVL_ROPE_HALF = 0, SVL_ROPE_ADJACENT = 1, SVL_ROPE_AXIAL = 2 } svl_rope_layout;
+
+/* Rows of heads: element c of head h of token t at
+ * t * token_stride + h * head_stride + c (strides in elements). */
+typedef struct {
+    const void *in;
+    void *out; /* may be `in` (same strides): rotated in place */
+    int64_t heads;
+    int64_t in_token_stride, in_head_stride;
+    int64_t out_token_stride, out_head_stride;
+} svl_rope_rows;
+
+/* Rotates pair j of every head by d_positions[t, pair_axis[j]] * inv_freq[j]
+ * (the product and its turns in 64 bits, so that far positions keep their
+ * fraction), in 32 bits, rounded once; columns from 2 * pairs on are copied.
+ * One or two tensors (queries and keys) in one launch. dtype SVL_F32 or
+ * SVL_BF16; 1..4 axes; inv_freq and pair_axis [pairs] on the host; head_dim at
+ * most 1024, pairs at most 256. Rows of `out` must not overlap others of `in`.
+ * Runs on the current device. */
+svl_status svl_rope_axes(const svl_rope_rows *tensors, int32_t n_tensors, int32_t dtype,
+                         const int32_t *d_positions, int64_t tokens, int32_t axes,
+                         int64_t head_dim, const float *inv_freq, const uint8_t *pair_axis,
+                         int64_t pairs, int32_t layout, void *stream);
+
+typedef struct svl_attention_plan svl_attention_plan;
+
+typedef struct {
+    int64_t num_heads, num_kv_heads; /* query head h reads KV head h / (heads / kv heads) */
+    int64_t head_dim;                /* 1..1024 */
+    int32_t dtype;                   /* SVL_F32 or SVL_BF16: queries, keys, values and output */
+    int32_t causal;                  /* non-zero: no keys after the query's position */
+    int64_t window;                  /* < 0: none, else |position - key| <= window */
+} svl_attention_shape;
+
+/* A batch of `documents` packed documents: document d has query rows
+ * q_offsets[d] .. q_offsets[d + 1] and key rows kv_offsets[d] ..
+ * kv_offsets[d + 1] (NULL: the same offsets); its last query stands at its
+ * last key, so query i has position i + keys - queries. Query and key rows may
+ * be none. A key j is visible to a query of its document at position p if it
+ * is one of the first prefix[d] keys (NULL: none), or if
+ * (not causal or j <= p) and (no window or |p - j| <= window). Offsets start
+ * at 0 or later and do not decrease; at most 2^31 - 1 rows. */
+svl_status svl_attention_plan_create(svl_ctx *ctx, const svl_attention_shape *shape,
+                                     const int64_t *q_offsets, const int64_t *kv_offsets,
+                                     const int64_t *prefix, int32_t documents,
+                                     svl_attention_plan **out);
+svl_status svl_attention_plan_destroy(svl_attention_plan *plan);
+/* Bytes of device workspace that a call needs (0: none), 16-byte aligned. */
+int64_t svl_attention_plan_workspace(const svl_attention_plan *plan);
+
+/* Strides in elements, as in svl_rope_rows; the last axis is contiguous. */
+typedef struct {
+    const void *q, *k, *v;
+    void *out;
+    float *lse; /* NULL, or [query rows, heads]: log of the sum of exponentials */
+    int64_t q_token_stride, q_head_stride;
+    int64_t k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride;
+    int64_t out_token_stride, out_head_stride;
+    float scale;         /* finite */
+    float soft_cap;      /* 0: none, else s = cap tanh(s / cap), cap > 0 and finite */
+    const float *slopes; /* NULL, or [heads] in HBM: s -= slope * |position - key| after the cap */
+} svl_attention_args;
+
+/* out = softmax(s) v over each query's visible keys, s = scale q . k with cap
+ * and bias; sums, maxima and probabilities' sums in 32 bits. A query without
+ * visible keys (or whose scores are all -inf) gives 0 and an lse of -inf.
+ * Query rows outside every document are left as they were, keys outside every
+ * document are not read, and a value that is masked for a query never reaches
+ * its output. `out` overlaps no input. */
+svl_status svl_masked_attention(const svl_attention_plan *plan, const svl_attention_args *args,
+                                void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- deterministic synthetic data (benchmark and tests) ------------------ */
 /* Counter-based SplitMix64: element i of stream s under seed k is
  * u = (splitmix64(k ^ (s * 0x9E3779B97F4A7C15) + i) >> 40) / 2^24 in [0, 1),

@@ -116,6 +116,9 @@ EXPORTED = [
     "svl_vector_index_size", "svl_vector_index_dimension", "svl_vector_rank",
     "svl_vector_rank_device", "svl_tensor_to_f32", "svl_bidirectional_attention_noalloc",
     "svl_measure_peaks", "svl_measure_fp64_peak", "svl_set_attention_path",
+    "svl_position_plan_create", "svl_position_plan_destroy", "svl_position_plan_tokens",
+    "svl_axis_positions", "svl_rope_axes", "svl_attention_plan_create",
+    "svl_attention_plan_destroy", "svl_attention_plan_workspace", "svl_masked_attention",
 ]
 
 _lib = None
