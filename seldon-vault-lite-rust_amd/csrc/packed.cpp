@@ -170,8 +170,11 @@ svl_status fill_attention(svl_attention_plan &plan, const int64_t *qo, const int
                           std::vector<AttnJoin> &join) {
     const svl_attention_shape &sh = plan.shape;
     const int64_t G = sh.num_heads / sh.num_kv_heads;
-    plan.tiles = masked_shape(sh.dtype == SVL_BF16, (int)sh.head_dim);
+    int64_t most = 0;
+    for (int32_t d = 0; d < documents; ++d) most = std::max(most, (qo[d + 1] - qo[d]) * G);
+    plan.tiles = masked_shape(sh.dtype == SVL_BF16, (int)sh.head_dim, most);
     const int64_t KT = plan.tiles.keys, BV = plan.tiles.vectors;
+    int64_t total = 0;  // key tiles of all groups
     for (int32_t d = 0; d < documents; ++d) {
         const int64_t ql = qo[d + 1] - qo[d], kl = ko[d + 1] - ko[d];
         const int64_t pre = prefix ? std::min(prefix[d], kl) : 0;
@@ -189,11 +192,37 @@ svl_status fill_attention(svl_attention_plan &plan, const int64_t *qo, const int
                 }
                 const int64_t pre_tiles = (pre + KT - 1) / KT;
                 const int64_t first = std::max(lo / KT, pre_tiles);
-                const int64_t tiles = pre_tiles + (hi >= lo ? std::max<int64_t>(hi / KT + 1 - first, 0) : 0);
+                const int64_t tiles =
+                    pre_tiles + (hi >= lo ? std::max<int64_t>(hi / KT + 1 - first, 0) : 0);
+                total += tiles;
+                // (keys past the last tile are never asked for, so main_key may pass them)
                 work.push_back({(int32_t)qo[d], (int32_t)ql, (int32_t)ko[d], (int32_t)kl,
                                 (int32_t)g, (int32_t)v0, (int32_t)pre, (int32_t)pre_tiles,
-                                (int32_t)(first * KT), 0, (int32_t)tiles, -1});
+                                (int32_t)std::min<int64_t>(first * KT, INT32_MAX), 0,
+                                (int32_t)tiles, -1});
             }
+    }
+    // Few groups leave CUs idle: their key tiles are split over workgroups, whose
+    // parts a second launch joins.
+    const int64_t target = BV == 32 ? 1280 : 512;
+    if (plan.tiles.dim > 0 && (int64_t)work.size() < target && total > (int64_t)work.size()) {
+        const int64_t each = std::max<int64_t>((total + target - 1) / target, 4);
+        std::vector<AttnWork> split;
+        int64_t slots = 0;
+        for (const AttnWork &w : work) {
+            const int64_t parts = std::max<int64_t>((w.t1 + each - 1) / each, 1);
+            if (parts > 1) join.push_back({w.q_row, w.q_len, w.kvh, w.v0, (int32_t)slots, (int32_t)parts});
+            for (int64_t i = 0; i < parts; ++i) {
+                AttnWork x = w;
+                x.t0 = (int32_t)(w.t1 * i / parts);
+                x.t1 = (int32_t)(w.t1 * (i + 1) / parts);
+                x.slot = parts > 1 ? (int32_t)(slots + i) : -1;
+                split.push_back(x);
+            }
+            if (parts > 1) slots += parts;
+        }
+        work.swap(split);
+        plan.workspace = slots * masked_slot(plan.tiles) * (int64_t)sizeof(float);
     }
     if (work.size() > INT32_MAX) return fail(SVL_LIMIT, "more than 2^31 - 1 work items");
     plan.n_work = (int32_t)work.size();

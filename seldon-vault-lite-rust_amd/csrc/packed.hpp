@@ -76,13 +76,16 @@ struct MaskedArgs {
     float *partial;
 };
 
-// Tile sizes that a plan is made for.
+// The kernel that a plan is made for, and its tiles.
 struct MaskedShape {
+    int dim;      // head dim that its tiles hold, 0: the kernel of one wave a query
     int vectors;  // query vectors per workgroup
     int keys;     // keys per tile
-    int width;    // floats per vector of a partial result: output, maximum, sum
 };
-MaskedShape masked_shape(bool bf16, int hd);
+// most: query vectors of the batch's largest document and KV head.
+MaskedShape masked_shape(bool bf16, int hd, int64_t most);
+// Floats of a slot of the workspace: outputs, maxima and sums of its vectors.
+inline int64_t masked_slot(const MaskedShape &s) { return (int64_t)s.vectors * (s.dim + 2); }
 hipError_t launch_masked_attention(const MaskedArgs &a, bool bf16, const MaskedShape &shape,
                                    hipStream_t s);
 

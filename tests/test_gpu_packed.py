@@ -296,14 +296,17 @@ def test_attention_values_hidden_from_some(nh, nkv, hd, dtype):
     n, bad = 200, 90
     plan = P.AttentionPlan([0, n], num_heads=nh, num_kv_heads=nkv, head_dim=hd, dtype=dtype,
                            causal=True)
-    q, k, v = (normal(rng, (n, h, hd), dtype)[0] for h in (nh, nkv, nkv))
-    clean, out = torch.empty_like(q), torch.empty_like(q)
-    P.masked_attention(plan, q, k, v, clean, 0.1)
+    (q, q64), (k, k64), (v, v64) = (normal(rng, (n, h, hd), dtype) for h in (nh, nkv, nkv))
+    out = torch.empty_like(q)
+    # rows before see neither, and may be summed another way beside such values: the bound of the
+    # 64-bit form holds for them either way
+    want, _, bound, _ = R.attention(q64, k64, v64, [0, n], [0, n], causal=True, scale=0.1,
+                                    bf16=dtype == BF16)
     for key, value in ((math.nan, math.nan), (1.0, math.inf), (math.inf, -math.inf)):
         kk, vv = k.clone(), v.clone()
         kk[bad], vv[bad] = key, value
         P.masked_attention(plan, q, kk, vv, out, 0.1)
-        assert torch.equal(out[:bad], clean[:bad])
+        within(host(out[:bad]), want[:bad], bound[:bad])
         assert not torch.isfinite(out[bad]).any()
 
 
@@ -332,7 +335,10 @@ def test_attention_keys_of_one_row():
 
 @pytest.mark.parametrize("dtype", TYPES)
 def test_attention_scores_past_the_range_of_exponentials(dtype):
-    """Scores of +-10^5: one key takes all the weight."""
+    """Scores of +-10^5: one key takes all the weight, v p / p. p need not be one (a kernel may keep
+    a maximum up to 2^8 behind), so the result is not v to the bit: in 32 bits the product of three
+    parts by three rounds at each of its six sums and leaves out 2 half steps, 1 / p is off by up
+    to 2 and the last product by one, 12 in all; in bfloat16 p and the result are rounded to it."""
     rng = np.random.default_rng(11)
     q, q64 = normal(rng, (70, 2, 64), dtype, 300.0)
     k, k64 = normal(rng, (70, 2, 64), dtype, 300.0)
@@ -347,7 +353,8 @@ def test_attention_scores_past_the_range_of_exponentials(dtype):
     want = v64[best, np.arange(2)[None]]
     got = host(out)
     assert np.isfinite(got).all() and clear.mean() > 0.8
-    np.testing.assert_array_equal(got[clear], want[clear])
+    rel = 12 * R.E32 if dtype == F32 else 2 * R.E16 * (1 + R.E16) + 12 * R.E32
+    within(got[clear], want[clear], rel * np.abs(want[clear]))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
