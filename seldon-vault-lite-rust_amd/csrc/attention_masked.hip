@@ -138,92 +138,89 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t (&p)[3]) {
     p[2] = pack_bf16(ra - __uint_as_float(p[1] << 16), rb - __uint_as_float(p[1] & 0xffff0000u));
 }
 
-// A tile's way from HBM to LDS: fetch() starts it, commit() ends it. `P`
-// planes of KT rows of D bfloat16 in LDS. Whole 16-byte chunks of bfloat16 rows
-// go there by DMA; rows of another alignment and float rows go through
-// registers (float ones are split on the way).
-template <class T, int P, int D, int KT, int THREADS, bool WHOLE, int (*SWIZZLE)(int)>
+// A tile's way from HBM to LDS: fetch() starts it, commit() ends it.
+//  * FROM_ROWS: whole 16-byte chunks of bfloat16 rows, by DMA.
+//  * FROM_PIECES: bfloat16 rows of any alignment, through registers.
+//  * FROM_PLANES: tiles that masked_planes_kernel has laid out, P planes of
+//    them as they lie in LDS, by DMA.
+enum TileSource { FROM_ROWS, FROM_PIECES, FROM_PLANES };
+
+template <class T, int P, int D, int KT, int THREADS, TileSource FROM, int (*SWIZZLE)(int)>
 struct TileCopy {
-    static constexpr int CHUNKS = KT * D / 8;          // of eight values
-    static constexpr int EACH = CHUNKS / THREADS;
-    static constexpr bool DMA = WHOLE && P == 1;
-    static_assert(CHUNKS % THREADS == 0, "tile");
-    static constexpr int OUT = (int)0x80000000;        // an offset out of range: reads zero
-    T reg[DMA ? 1 : EACH * 8];
+    static constexpr int EACH = (FROM == FROM_PLANES ? P : 1) * KT * D / 8 / THREADS;  // chunks of a thread
+    static_assert(KT * D / 8 % THREADS == 0, "tile");
+    static constexpr int OUT = (int)0x80000000;  // an offset out of range: reads zero
+    __bf16 reg[FROM == FROM_PIECES ? EACH * 8 : 1];
+    // Offsets are kept where there is room, else found anew for each tile (at
+    // 256 dims the registers are worth more than the few instructions).
+    static constexpr bool KEPT = FROM == FROM_ROWS && D < 256;
+    int kept[KEPT ? EACH : 1];
+
+    __device__ __forceinline__ static int offset(int i, int lane, int ld, int hd) {
+        const int c = ((int)threadIdx.x >> 6) * (64 * EACH) + 64 * i + lane;
+        if constexpr (FROM == FROM_PLANES) return c * 16;
+        const int r = c / (D / 8), dim = 8 * ((c % (D / 8)) ^ SWIZZLE(r));
+        return FROM == FROM_PIECES || dim < hd ? (r * ld + dim) * 2 : OUT;
+    }
+    __device__ __forceinline__ void init(int ld, int hd) {
+        if constexpr (KEPT) {
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) kept[i] = offset(i, (int)threadIdx.x & 63, ld, hd);
+        }
+    }
 
     // chunk that this thread moves i-th: a wave's DMA fills 1 KB of LDS in a row
     __device__ __forceinline__ static int place(int i) {
         return ((int)threadIdx.x >> 6) * (64 * EACH) + 64 * i + ((int)threadIdx.x & 63);
     }
     // rows: rows of the tile that exist
-    __device__ __forceinline__ void fetch(const T *base, int ld, int hd, int rows, __bf16 *lds) {
+    __device__ __forceinline__ void fetch(const void *base, int ld, int hd, int rows, __bf16 *lds) {
+        const int bytes = FROM == FROM_PLANES ? P * KT * D * 2 : ((rows - 1) * ld + hd) * 2;
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-            (void *)uniform((T *)base), (short)0, uniform(((rows - 1) * ld + hd) * (int)sizeof(T)),
-            0x00020000);
+            uniform((char *)base), (short)0, uniform(bytes), 0x00020000);
         const int wave = uniform((int)threadIdx.x >> 6);
-        // found anew for each tile: the registers are worth more than the few
-        // instructions
         int lane = (int)threadIdx.x & 63;
-        asm volatile("" : "+v"(lane));
+        if constexpr (!KEPT) asm volatile("" : "+v"(lane));
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
-            const int c = wave * (64 * EACH) + 64 * i + lane;
-            const int r = c / (D / 8), dim = 8 * ((c % (D / 8)) ^ SWIZZLE(r));
-            const int off = (r * ld + dim) * (int)sizeof(T);
-            if constexpr (DMA) {
+            int off;
+            if constexpr (KEPT) off = kept[i];
+            else off = offset(i, lane, ld, hd);
+            if constexpr (FROM == FROM_PIECES) {
+                const int c = wave * (64 * EACH) + 64 * i + lane, r = c / (D / 8);
+                const int dim = 8 * ((c % (D / 8)) ^ SWIZZLE(r));
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    reg[8 * i + e] = __builtin_bit_cast(
+                        __bf16, __builtin_amdgcn_raw_buffer_load_b16(
+                                    rs, dim + e < hd ? off + 2 * e : OUT, 0, 0));
+            } else {
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
                     rs, (__attribute__((address_space(3))) void *)(lds + (wave * EACH + i) * 512),
-                    16, dim < hd ? off : OUT, 0, 0, 0);
-            } else if constexpr (WHOLE) {  // float
-#pragma unroll
-                for (int q = 0; q < 8; q += 4) {
-                    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(
-                        rs, dim + q < hd ? off + 4 * q : OUT, 0, 0);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) reg[8 * i + q + e] = __uint_as_float(v[e]);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int o = dim + e < hd ? off + e * (int)sizeof(T) : OUT;
-                    if constexpr (sizeof(T) == 2)
-                        reg[8 * i + e] = __builtin_bit_cast(
-                            __bf16, __builtin_amdgcn_raw_buffer_load_b16(rs, o, 0, 0));
-                    else
-                        reg[8 * i + e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, o, 0, 0));
-                }
+                    16, off, 0, 0, 0);
             }
         }
     }
     __device__ __forceinline__ void commit(__bf16 *lds) {
-        if constexpr (DMA) {
+        if constexpr (FROM != FROM_PIECES) {
             wait_vmcnt<0>();
         } else {
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
-                u32x4 pl[P];
+                bf16x8 v;
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    if constexpr (P == 1) {
-                        pl[0][e / 2] = __builtin_bit_cast(uint32_t, bf16x2{reg[8 * i + e], reg[8 * i + e + 1]});
-                    } else {
-                        uint32_t x[3];
-                        split3<false>(reg[8 * i + e], reg[8 * i + e + 1], x);
-#pragma unroll
-                        for (int p = 0; p < P; ++p) pl[p][e / 2] = x[p];
-                    }
-                }
-#pragma unroll
-                for (int p = 0; p < P; ++p) *(u32x4 *)(lds + p * KT * D + place(i) * 8) = pl[p];
+                for (int e = 0; e < 8; ++e) v[e] = reg[8 * i + e];
+                *(bf16x8 *)(lds + place(i) * 8) = v;
             }
         }
     }
-    // Whether this thread's part of a landed tile holds a non-finite value
-    // (high parts tell).
-    __device__ __forceinline__ bool non_finite(const __bf16 *lds) const {
+    // Whether this thread's part of a landed tile holds a non-finite value (of
+    // three planes the first tells).
+    __device__ __forceinline__ static bool non_finite(const __bf16 *lds) {
         uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
+            if (place(i) * 8 >= KT * D) continue;
             const u32x4 v = *(const u32x4 *)(lds + place(i) * 8);
 #pragma unroll
             for (int e = 0; e < 4; ++e) any |= (v[e] & 0x7fff7fffu) + 0x00800080u;
@@ -231,6 +228,49 @@ struct TileCopy {
         return (any & 0x80008000u) != 0;
     }
 };
+
+// Float keys and values as planes: three bfloat16 parts of a tile of KT keys of
+// a document and KV head, each in the order of LDS, keys and dims past the end
+// zero. Done once a call: splitting them in every workgroup that reads them was
+// a third of the vector work of the tile kernel (documents of 64-512 tokens, 3
+// heads of 256: 214 us against FLOAT_US).
+template <int D, int KT>
+__global__ __launch_bounds__(256) void masked_planes_kernel(MaskedArgs a) {
+    const AttnTiles w = a.tiles[blockIdx.x];
+    const bool values = blockIdx.y != 0;
+    const float *base = (const float *)(values ? a.v : a.k) +
+                        (int64_t)w.k_row * (values ? a.v_tok : a.k_tok) +
+                        w.kvh * (values ? a.v_head : a.k_head);
+    const int64_t ld = values ? a.v_tok : a.k_tok;
+    __bf16 *out = (__bf16 *)a.planes + ((int64_t)blockIdx.x * 2 + values) * (3 * KT * D);
+    for (int c = threadIdx.x; c < KT * D / 8; c += 256) {
+        const int r = c / (D / 8);
+        const int dim = 8 * ((c % (D / 8)) ^ (values ? value_swizzle<D>(r) : key_swizzle<D>(r)));
+        float x[8];
+        const float *row = base + r * ld + dim;
+        if (r < w.rows && a.whole && dim + 8 <= a.hd) {
+            const f32x4 u = *(const f32x4 *)row, v = *(const f32x4 *)(row + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = u[e];
+                x[4 + e] = v[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = r < w.rows && dim + e < a.hd ? row[e] : 0.f;
+        }
+        u32x4 pl[3];
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            uint32_t y[3];
+            split3<false>(x[e], x[e + 1], y);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) pl[p][e / 2] = y[p];
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *(u32x4 *)(out + p * KT * D + c * 8) = pl[p];
+    }
+}
 
 // Four keys x 16 dims of bfloat16 read transposed (a lane's 8-byte piece: key
 // (lane % 16) / 4 of the four, dims 4 (lane % 4) ..): the lane receives dim
@@ -259,6 +299,16 @@ constexpr float TANH_C0 = -0.33333331f, TANH_C1 = 0.13333082f, TANH_C2 = -0.0539
 // tanh y = 1 - 2 / (e^2y + 1) loses the low bits of a small y (an absolute
 // error of 2^-24): float scores take the series y + y^3 P(y^2) below 0.55
 // (Chebyshev fit of tanh(y) / y, error 4e-8 there).
+// Max / sum over the four 16-lane groups of a wave.
+__device__ __forceinline__ float group_max4(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return other_half_max(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+}
+__device__ __forceinline__ float group_sum4(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return other_half_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
+}
+
 template <bool EXACT>
 __device__ __forceinline__ float capped(float s, float to2x, float capl) {
     const float z = s * to2x;
@@ -277,9 +327,9 @@ __device__ __forceinline__ float capped(float s, float to2x, float capl) {
     return t;
 }
 
-// A workgroup takes WAVES * 32 query vectors of one document and KV head: the
-// heads that share a KV head are vectors beside each other, so a tile of keys
-// serves all of them. Keys stream through LDS in tiles of KT.
+// A workgroup takes WAVES / DS * 32 query vectors of one document and KV head:
+// the heads that share a KV head are vectors beside each other, so a tile of
+// keys serves all of them. Keys stream through LDS in tiles of KT.
 //  * S^T = K Q^T on 32x32x16 MFMAs, queries in registers: a lane holds 16 of
 //    a block's 32 keys for one query, so that maximum and sum are a lane's own
 //    but for one exchange with lane ^ 32.
@@ -288,26 +338,37 @@ __device__ __forceinline__ float capped(float s, float to2x, float capl) {
 //    is read transposed in the same order.
 //  * The running maximum moves only when a query's grows by more than 2^8, so
 //    outputs are rarely rescaled.
-//  * One LDS buffer each for K and V: V(t) comes in under the scores of tile
-//    t, K(t + 1) under its softmax and P V; two barriers a tile.
+//  * STAGES = 2: a tile's K and V come in under the whole tile before, one
+//    barrier a tile. STAGES = 1, where LDS holds no more: V(t) comes in under
+//    the scores of tile t, K(t + 1) under its softmax and P V; two barriers.
+//  * DS = 2: two waves share 32 queries, each with half of the dims of scores
+//    (summed through LDS) and output, where one wave's registers would leave a
+//    SIMD to a single wave (float rows: three parts of every query; 256 dims
+//    311 us with one wave, 214 us with two).
 // P = 1: bfloat16 operands; weights are rounded to bfloat16 for the product
 // with V (a relative 2^-8 of each, the output's own step); their sum is taken
 // before, so that the lse keeps its 32 bits.
 // P = 3: float operands as three bfloat16 parts; of the nine products the six
 // above 2^-24 are taken, the five small ones in an accumulator of their own.
-template <class T, int P, int D, int KT, int WAVES, bool WHOLE, bool CAP, int MINB>
-__global__ __launch_bounds__(64 * WAVES, MINB) void masked_tile_kernel(MaskedArgs a) {
+template <class T, int P, int D, int KT, int WAVES, int DS, int STAGES, TileSource FROM, bool CAP,
+          int MINW>
+__global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int NB = D / 16, NT = D / 32, NK = KT / 32;
-    __shared__ __bf16 Ks[P * KT * D];
-    __shared__ __bf16 Vs[P * KT * D];
+    constexpr int DW = D / DS;  // dims of a wave
+    constexpr int NB = DW / 16, NT = DW / 32, NK = KT / 32, VECTORS = 32 * WAVES / DS;
+    // one object a stage, chosen at compile time: the compiler then sees that
+    // the DMA into one does not touch the reads of the other
+    __shared__ __bf16 K0[P * KT * D], V0[P * KT * D];
+    __shared__ __bf16 K1[STAGES > 1 ? P * KT * D : 8], V1[STAGES > 1 ? P * KT * D : 8];
+    __shared__ f32x4 Sx[DS > 1 ? WAVES * NK * 4 * 64 : 1];  // the waves' parts of the scores
     __shared__ int dirty;  // 1 + the tile whose values hold a non-finite one
     const AttnWork w = a.work[blockIdx.x];
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
     const int l32 = lane & 31, h = lane >> 5;
     const int G = a.heads / a.kv_heads;
     const int nvec = w.q_len * G;
-    const int wv0 = w.v0 + wave * 32;          // this wave's first vector
+    const int dim0 = (wave % DS) * DW;
+    const int wv0 = w.v0 + wave / DS * 32;     // this wave's first vector
     const bool some = wv0 < nvec;              // ... and whether it has any
     const int vec = min(wv0 + l32, nvec - 1);
     const bool valid = wv0 + l32 < nvec;
@@ -315,7 +376,7 @@ __global__ __launch_bounds__(64 * WAVES, MINB) void masked_tile_kernel(MaskedArg
     const int shift = w.k_len - w.q_len;
     const int p = qi + shift;
     const int p_lo = min(wv0, nvec - 1) / G + shift, p_hi = min(wv0 + 31, nvec - 1) / G + shift;
-    const int wg_lo = w.v0 / G + shift, wg_hi = min(w.v0 + 32 * WAVES - 1, nvec - 1) / G + shift;
+    const int wg_lo = w.v0 / G + shift, wg_hi = min(w.v0 + VECTORS - 1, nvec - 1) / G + shift;
 
     // a query's keys besides the prefix: lo .. hi
     auto first_key = [&](int pos) { return a.window >= 0 ? (int)max((int64_t)pos - a.window, (int64_t)0) : 0; };
@@ -326,6 +387,10 @@ __global__ __launch_bounds__(64 * WAVES, MINB) void masked_tile_kernel(MaskedArg
         return (int)max(k, (int64_t)-1);
     };
     const int lo = first_key(p), hi = last_key(p);
+    // the wave's: any of its queries, all of them; and all of the workgroup's
+    const int any_lo = first_key(p_lo), any_hi = last_key(p_hi);
+    const int all_lo = first_key(p_hi), all_hi = last_key(p_lo);
+    const int wg_all_lo = first_key(wg_hi), wg_all_hi = last_key(wg_lo);
 
     // scores: sign of the scale into the queries, its size into the exponent
     const float size = fabsf(a.scale);
@@ -335,9 +400,9 @@ __global__ __launch_bounds__(64 * WAVES, MINB) void masked_tile_kernel(MaskedArg
         const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const int d = 16 * b + 8 * h;
+            const int d = dim0 + 16 * b + 8 * h;
             T x[8];
-            if constexpr (WHOLE) {
+            if (a.whole) {
                 constexpr int N = 16 / sizeof(T);
 #pragma unroll
                 for (int i = 0; i < 8; i += N) {
@@ -381,227 +446,275 @@ __global__ __launch_bounds__(64 * WAVES, MINB) void masked_tile_kernel(MaskedArg
     float m_ref = -INFINITY, l_run = 0.f;
 
     const int ldk = (int)a.k_tok, ldv = (int)a.v_tok;
-    const T *kbase = (const T *)a.k + w.k_row * a.k_tok + w.kvh * a.k_head;
-    const T *vbase = (const T *)a.v + w.k_row * a.v_tok + w.kvh * a.v_head;
-    TileCopy<T, P, D, KT, 64 * WAVES, WHOLE, key_swizzle<D>> kc;
-    TileCopy<T, P, D, KT, 64 * WAVES, WHOLE, value_swizzle<D>> vc;
+    const __bf16 *kbase = FROM == FROM_PLANES ? (const __bf16 *)a.planes + (int64_t)w.tile0 * (2 * P * KT * D)
+                                              : (const __bf16 *)a.k + w.k_row * a.k_tok + w.kvh * a.k_head;
+    const __bf16 *vbase = FROM == FROM_PLANES ? kbase + P * KT * D
+                                              : (const __bf16 *)a.v + w.k_row * a.v_tok + w.kvh * a.v_head;
+    TileCopy<T, P, D, KT, 64 * WAVES, FROM, key_swizzle<D>> kc;
+    TileCopy<T, P, D, KT, 64 * WAVES, FROM, value_swizzle<D>> vc;
+    kc.init(ldk, a.hd);
+    vc.init(ldv, a.hd);
     auto key_of = [&](int t) { return t < w.pre_tiles ? t * KT : w.main_key + (t - w.pre_tiles) * KT; };
-    auto fetch_k = [&](int k0) {
-        kc.fetch(kbase + (int64_t)k0 * ldk, ldk, a.hd, min(KT, w.k_len - k0), Ks);
+    auto fetch_k = [&](int k0, __bf16 *to) {
+        kc.fetch(FROM == FROM_PLANES ? kbase + (int64_t)k0 * (2 * P * D) : kbase + (int64_t)k0 * ldk,
+                 ldk, a.hd, min(KT, w.k_len - k0), to);
     };
-    auto fetch_v = [&](int k0) {
-        vc.fetch(vbase + (int64_t)k0 * ldv, ldv, a.hd, min(KT, w.k_len - k0), Vs);
+    auto fetch_v = [&](int k0, __bf16 *to) {
+        vc.fetch(FROM == FROM_PLANES ? vbase + (int64_t)k0 * (2 * P * D) : vbase + (int64_t)k0 * ldv,
+                 ldv, a.hd, min(KT, w.k_len - k0), to);
     };
     // Lane addresses, in elements: K row l32 of a block at chunk h, V row
     // (lane % 16) / 4 of four at its chunk of a 32-dim tile. Rows start at
     // multiples of D, so another chunk (a multiple of 2 or 4 further before the
     // swizzle) is an exclusive or of the offset; it is done as each fragment is
     // read (kept in registers, the addresses would spill).
-    int koff = l32 * D + ((h ^ key_swizzle<D>(l32)) << 3);
+    int koff = l32 * D + (((dim0 / 8 + h) ^ key_swizzle<D>(l32)) << 3);
     const int vr = 4 * h + ((lane & 15) >> 2);
-    int voff = vr * D + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ value_swizzle<D>(vr)) << 3) +
+    int voff = vr * D + (((dim0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ value_swizzle<D>(vr)) << 3) +
                4 * (lane & 1);
 
-    if (threadIdx.x == 0) dirty = 0;
-    bool redo = false;
-    if (w.t0 < w.t1) {
-        fetch_k(key_of(w.t0));
-        kc.commit(Ks);
-    }
-    __syncthreads();
-    for (int t = w.t0; t < w.t1; ++t) {
-        const int k0 = key_of(t);
-        asm volatile("" : "+v"(koff), "+v"(voff));  // no hoisting of what follows from them
-        fetch_v(k0);
-        // what of the tile this wave's queries see
-        const bool in_prefix = k0 < w.prefix;
-        const bool seen = some && (in_prefix || (k0 <= last_key(p_hi) && k0 + KT > first_key(p_lo)));
-        const bool all = k0 + KT <= w.prefix ||
-                         (k0 >= first_key(p_hi) && k0 + KT - 1 <= last_key(p_lo));
-        f32x16 s[NK];
-        if (seen) {
+    f32x16 s[NK];
+    auto scores = [&](const __bf16 *Ks) {
 #pragma unroll
-            for (int kb = 0; kb < NK; ++kb) {
-                f32x16 big, rest;
+        for (int kb = 0; kb < NK; ++kb) {
+            f32x16 big, rest;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) big[r] = rest[r] = 0.f;
+            for (int r = 0; r < 16; ++r) big[r] = rest[r] = 0.f;
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const __bf16 *at = Ks + (koff ^ (16 * b));
-                    bf16x8 k[P];
+            for (int b = 0; b < NB; ++b) {
+                const __bf16 *at = Ks + (koff ^ (16 * b));
+                bf16x8 k[P];
 #pragma unroll
-                    for (int i = 0; i < P; ++i)
-                        k[i] = *(const bf16x8 *)(at + i * KT * D + kb * 32 * D);
-                    big = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[0], q[0][b], big, 0, 0, 0);
-                    if constexpr (P == 3) {
-                        rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[2], q[0][b], rest, 0, 0, 0);
-                        rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[0], q[P - 1][b], rest, 0, 0, 0);
-                        rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[1], q[P / 2][b], rest, 0, 0, 0);
-                        rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[1], q[0][b], rest, 0, 0, 0);
-                        rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[0], q[P / 2][b], rest, 0, 0, 0);
-                    }
-                }
+                for (int i = 0; i < P; ++i) k[i] = *(const bf16x8 *)(at + i * KT * D + kb * 32 * D);
+                big = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[0], q[0][b], big, 0, 0, 0);
                 if constexpr (P == 3) {
-                    // an infinite score is what its high parts give (the others' products
-                    // with it may be 0 * inf)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) big[r] += isfinite(big[r]) ? rest[r] : 0.f;
+                    rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[2], q[0][b], rest, 0, 0, 0);
+                    rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[0], q[P - 1][b], rest, 0, 0, 0);
+                    rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[1], q[P / 2][b], rest, 0, 0, 0);
+                    rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[1], q[0][b], rest, 0, 0, 0);
+                    rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[0], q[P / 2][b], rest, 0, 0, 0);
                 }
-                s[kb] = big;
+            }
+            if constexpr (P == 3) {
+                // an infinite score is what its high parts give (the others' products
+                // with it may be 0 * inf)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) big[r] += isfinite(big[r]) ? rest[r] : 0.f;
+            }
+            s[kb] = big;
+            if constexpr (DS > 1) {
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    Sx[((wave * NK + kb) * 4 + r / 4) * 64 + lane] =
+                        f32x4{big[r], big[r + 1], big[r + 2], big[r + 3]};
             }
         }
-        vc.commit(Vs);
-        // Values hidden from some of the workgroup's queries must not reach them
-        // through a product 0 * inf.
-        const bool mixed = !(k0 + KT <= w.prefix ||
-                             (k0 >= first_key(wg_hi) &&
-                              min(k0 + KT, w.k_len) - 1 <= last_key(wg_lo)));
-        if (mixed && __ballot(vc.non_finite(Vs)) != 0 && lane == 0) dirty = t + 1;
-        __syncthreads();  // V has landed; no wave reads K any more
-        if (mixed && uniform(*(volatile int *)&dirty) == t + 1) {
-            redo = true;
-            break;
+    };
+    auto weigh = [&](const __bf16 *Vs, int k0, bool all) {
+        if constexpr (DS > 1) {
+#pragma unroll
+            for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const f32x4 x = Sx[(((wave ^ 1) * NK + kb) * 4 + r / 4) * 64 + lane];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[kb][r + e] += x[e];
+                }
         }
-        if (t + 1 < w.t1) fetch_k(key_of(t + 1));
-        if (seen) {
-            float tmax = -INFINITY;
-            auto score = [&](int kb, int r) {  // log2 units
-                float x = CAP ? capped<P == 3>(s[kb][r], to2x, capl) : s[kb][r] * to_log2;
-                return x;
-            };
-            if (CAP || a.slopes || !all) {
+        float tmax = -INFINITY, mul = to_log2;
+        if (CAP || a.slopes || !all) {  // to log2 units first
+            mul = 1.f;
+#pragma unroll
+            for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    s[kb][r] = CAP ? capped<P == 3>(s[kb][r], to2x, capl) : s[kb][r] * to_log2;
+            if (a.slopes) {
                 const float d0 = (float)(p - k0 - 4 * h);
 #pragma unroll
                 for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[kb][r] = score(kb, r);
-                if (a.slopes) {
-#pragma unroll
-                    for (int kb = 0; kb < NK; ++kb)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            s[kb][r] = __builtin_fmaf(
-                                -slope, fabsf(d0 - (float)(32 * kb + 8 * (r >> 2) + (r & 3))), s[kb][r]);
-                }
-                if (!all) {
-#pragma unroll
-                    for (int kb = 0; kb < NK; ++kb)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int key = k0 + 32 * kb + 8 * (r >> 2) + 4 * h + (r & 3);
-                            s[kb][r] = key < w.prefix || (key >= lo && key <= hi) ? s[kb][r] : -INFINITY;
-                        }
-                }
+                    for (int r = 0; r < 16; ++r)
+                        s[kb][r] = __builtin_fmaf(
+                            -slope, fabsf(d0 - (float)(32 * kb + 8 * (r >> 2) + (r & 3))), s[kb][r]);
+            }
+            if (!all) {
 #pragma unroll
                 for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[kb][r]);
-            } else {
-#pragma unroll
-                for (int kb = 0; kb < NK; ++kb)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[kb][r]);
-                tmax *= to_log2;
+                    for (int r = 0; r < 16; ++r) {
+                        const int key = k0 + 32 * kb + 8 * (r >> 2) + 4 * h + (r & 3);
+                        s[kb][r] = key < w.prefix || (key >= lo && key <= hi) ? s[kb][r] : -INFINITY;
+                    }
             }
-            const float mul = CAP || a.slopes || !all ? 1.f : to_log2;
-            tmax = other_half_max(tmax);
-            const bool grow = tmax > m_ref + 8.f;
-            if (__ballot(grow)) {
-                const float m_new = grow ? tmax : m_ref;
-                const float alpha = m_ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref - m_new);
-                l_run *= alpha;
+        }
 #pragma unroll
-                for (int d = 0; d < NT; ++d) o[d] = o[d] * alpha;
-                m_ref = m_new;
+        for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[kb][r]);
+        tmax = other_half_max(tmax) * mul;
+        const bool grow = tmax > m_ref + 8.f;
+        if (__ballot(grow)) {
+            const float m_new = grow ? tmax : m_ref;
+            const float alpha = m_ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref - m_new);
+            l_run *= alpha;
+#pragma unroll
+            for (int d = 0; d < NT; ++d) o[d] = o[d] * alpha;
+            m_ref = m_new;
+        }
+        const float base = m_ref == -INFINITY ? 0.f : -m_ref;
+        bf16x8 pr[P][NK][2];
+        float psum = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * u + i], mul, base));
+                    psum += e[i];
+                }
+                if constexpr (P == 1) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) pr[0][kb][u][i] = (__bf16)e[i];
+                } else {
+                    u32x4 pl[P];
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        uint32_t x[3];
+                        split3<true>(e[i], e[i + 1], x);
+#pragma unroll
+                        for (int j = 0; j < P; ++j) pl[j][i / 2] = x[j];
+                    }
+#pragma unroll
+                    for (int j = 0; j < P; ++j) pr[j][kb][u] = __builtin_bit_cast(bf16x8, pl[j]);
+                }
             }
-            const float base = m_ref == -INFINITY ? 0.f : -m_ref;
-            bf16x8 pr[P][NK][2];
-            float psum = 0.f;
+        l_run += other_half_sum(psum);
+#pragma unroll
+        for (int d = 0; d < NT; ++d) {
+            const __bf16 *tile = Vs + (voff ^ (32 * d));
+            f32x16 rest;
+            if constexpr (P == 3) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) rest[r] = 0.f;
+            }
 #pragma unroll
             for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    float e[8];
+                    bf16x8 v[P];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * u + i], mul, base));
-                    if constexpr (P == 1) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            psum += e[i];
-                            pr[0][kb][u][i] = (__bf16)e[i];
-                        }
-                    } else {
-                        u32x4 pl[P];
-#pragma unroll
-                        for (int i = 0; i < 8; i += 2) {
-                            uint32_t x[3];
-                            psum += e[i];
-                            psum += e[i + 1];
-                            split3<true>(e[i], e[i + 1], x);
-#pragma unroll
-                            for (int j = 0; j < P; ++j) pl[j][i / 2] = x[j];
-                        }
-#pragma unroll
-                        for (int j = 0; j < P; ++j) pr[j][kb][u] = __builtin_bit_cast(bf16x8, pl[j]);
+                    for (int i = 0; i < P; ++i) {
+                        const __bf16 *at = tile + i * KT * D + (32 * kb + 16 * u) * D;
+                        v[i] = __builtin_shufflevector(read_transposed_bf16(at),
+                                                       read_transposed_bf16(at + 8 * D), 0, 1, 2,
+                                                       3, 4, 5, 6, 7);
+                    }
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[0], pr[0][kb][u], o[d], 0, 0, 0);
+                    if constexpr (P == 3) {
+                        rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[2], pr[0][kb][u], rest, 0, 0, 0);
+                        rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[0], pr[P - 1][kb][u], rest, 0, 0, 0);
+                        rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[1], pr[P / 2][kb][u], rest, 0, 0, 0);
+                        rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[1], pr[0][kb][u], rest, 0, 0, 0);
+                        rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[0], pr[P / 2][kb][u], rest, 0, 0, 0);
                     }
                 }
-            l_run += other_half_sum(psum);
-#pragma unroll
-            for (int d = 0; d < NT; ++d) {
-                const __bf16 *tile = Vs + (voff ^ (32 * d));
-                f32x16 rest;
-                if constexpr (P == 3) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) rest[r] = 0.f;
-                }
-#pragma unroll
-                for (int kb = 0; kb < NK; ++kb)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        bf16x8 v[P];
-#pragma unroll
-                        for (int i = 0; i < P; ++i) {
-                            const __bf16 *at = tile + i * KT * D + (32 * kb + 16 * u) * D;
-                            v[i] = __builtin_shufflevector(read_transposed_bf16(at),
-                                                           read_transposed_bf16(at + 8 * D), 0, 1, 2,
-                                                           3, 4, 5, 6, 7);
-                        }
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[0], pr[0][kb][u], o[d], 0, 0, 0);
-                        if constexpr (P == 3) {
-                            rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[2], pr[0][kb][u], rest, 0, 0, 0);
-                            rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[0], pr[P - 1][kb][u], rest, 0, 0, 0);
-                            rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[1], pr[P / 2][kb][u], rest, 0, 0, 0);
-                            rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[1], pr[0][kb][u], rest, 0, 0, 0);
-                            rest = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[0], pr[P / 2][kb][u], rest, 0, 0, 0);
-                        }
-                    }
-                if constexpr (P == 3) o[d] = o[d] + rest;
-            }
+            if constexpr (P == 3) o[d] = o[d] + rest;
         }
-        if (t + 1 < w.t1) kc.commit(Ks);
-        __syncthreads();  // K has landed; no wave reads V any more
+    };
+
+    if (threadIdx.x == 0) dirty = 0;
+    bool redo = false;
+    // V(t) has landed in the thread's part: whether values that are hidden from
+    // some of the workgroup's queries are finite. They must not reach those
+    // queries through a product 0 * inf.
+    auto inspect = [&](const __bf16 *Vs, int t, int k0) {
+        const bool mixed = !(k0 + KT <= w.prefix ||
+                             (k0 >= wg_all_lo && min(k0 + KT, w.k_len) - 1 <= wg_all_hi));
+        if (mixed && __ballot(vc.non_finite(Vs)) != 0 && lane == 0) dirty = t + 1;
+        return mixed;
+    };
+    // after a barrier: true where they are not, and the rows are to be redone
+    auto spoilt = [&](bool mixed, int t) {
+        redo = mixed && uniform(*(volatile int *)&dirty) == t + 1;
+        return redo;
+    };
+    auto sees = [&](int k0) { return some && (k0 < w.prefix || (k0 <= any_hi && k0 + KT > any_lo)); };
+    auto sees_all = [&](int k0) {
+        return k0 + KT <= w.prefix || (k0 >= all_lo && k0 + KT - 1 <= all_hi);
+    };
+    if constexpr (STAGES == 2) {
+        auto step = [&](int t, __bf16 *Ks, __bf16 *Vs, __bf16 *Kn, __bf16 *Vn) {
+            const int k0 = key_of(t);
+            asm volatile("" : "+v"(koff), "+v"(voff));  // no hoisting of what follows from them
+            kc.commit(Ks);
+            vc.commit(Vs);
+            const bool mixed = inspect(Vs, t, k0);
+            __syncthreads();  // tile t has landed; no wave reads tile t - 1 any more
+            if (spoilt(mixed, t)) return;
+            if (t + 1 < w.t1) {
+                fetch_k(key_of(t + 1), Kn);
+                fetch_v(key_of(t + 1), Vn);
+            }
+            const bool seen = sees(k0);
+            if (seen) scores(Ks);
+            if constexpr (DS > 1) __syncthreads();  // the other wave's part of the scores
+            if (seen) weigh(Vs, k0, sees_all(k0));
+        };
+        if (w.t0 < w.t1) {
+            fetch_k(key_of(w.t0), K0);
+            fetch_v(key_of(w.t0), V0);
+        }
+        for (int t = w.t0; t < w.t1; t += 2) {
+            step(t, K0, V0, K1, V1);
+            if (redo || t + 1 >= w.t1) break;
+            step(t + 1, K1, V1, K0, V0);
+            if (redo) break;
+        }
+    } else {
+        if (w.t0 < w.t1) {
+            fetch_k(key_of(w.t0), K0);
+            kc.commit(K0);
+        }
+        __syncthreads();
+        for (int t = w.t0; t < w.t1; ++t) {
+            const int k0 = key_of(t);
+            asm volatile("" : "+v"(koff), "+v"(voff));
+            fetch_v(k0, V0);
+            const bool seen = sees(k0);
+            if (seen) scores(K0);
+            vc.commit(V0);
+            const bool mixed = inspect(V0, t, k0);
+            __syncthreads();  // V has landed; no wave reads K any more
+            if (spoilt(mixed, t)) break;
+            if (t + 1 < w.t1) fetch_k(key_of(t + 1), K0);
+            if (seen) weigh(V0, k0, sees_all(k0));
+            if (t + 1 < w.t1) kc.commit(K0);
+            __syncthreads();  // K has landed; no wave reads V any more
+        }
     }
 
-    float *part = w.slot < 0 ? nullptr : a.partial + (int64_t)w.slot * (32 * WAVES * (D + 2));
+    float *part = w.slot < 0 ? nullptr : a.partial + (int64_t)w.slot * (VECTORS * (D + 2));
     if (redo) {
-        for (int i = wave * 32; i < wave * 32 + 32 && w.v0 + i < nvec; ++i)
+        for (int i = wave; i < VECTORS && w.v0 + i < nvec; i += WAVES)
             masked_row<T, D / 64>(a, w, w.v0 + i, KT, part ? part + i * D : nullptr,
-                                  part ? part + 32 * WAVES * D + 2 * i : nullptr);
+                                  part ? part + VECTORS * D + 2 * i : nullptr);
         return;
     }
     if (!valid) return;
-    const int local = wave * 32 + l32;
+    const int local = wave / DS * 32 + l32;
     if (part) {
 #pragma unroll
         for (int d = 0; d < NT; ++d)
 #pragma unroll
             for (int r = 0; r < 16; r += 4)
-                *(f32x4 *)(part + local * D + 32 * d + 2 * r + 4 * h) =
+                *(f32x4 *)(part + local * D + dim0 + 32 * d + 2 * r + 4 * h) =
                     f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
-        if (h == 0) {
-            part[32 * WAVES * D + 2 * local] = m_ref;
-            part[32 * WAVES * D + 2 * local + 1] = l_run;
+        if (h == 0 && dim0 == 0) {
+            part[VECTORS * D + 2 * local] = m_ref;
+            part[VECTORS * D + 2 * local + 1] = l_run;
         }
         return;
     }
@@ -612,11 +725,11 @@ __global__ __launch_bounds__(64 * WAVES, MINB) void masked_tile_kernel(MaskedArg
     for (int d = 0; d < NT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
-            const int dim = 32 * d + 2 * r + 4 * h;
+            const int dim = dim0 + 32 * d + 2 * r + 4 * h;
             typename Row<T, 4>::type y;
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = (T)(l_run == 0.f ? 0.f : o[d][r + e] * inv);
-            if constexpr (WHOLE) {
+            if (a.whole) {
                 if (dim < a.hd) *(typename Row<T, 4>::type *)(row + dim) = y;
             } else {
 #pragma unroll
@@ -624,58 +737,308 @@ __global__ __launch_bounds__(64 * WAVES, MINB) void masked_tile_kernel(MaskedArg
                     if (dim + e < a.hd) row[dim + e] = y[e];
             }
         }
-    if (a.lse && h == 0)
+    if (a.lse && h == 0 && dim0 == 0)
         a.lse[qrow * a.heads + head] =
             l_run == 0.f ? -INFINITY : (m_ref + __builtin_amdgcn_logf(l_run)) * 0.6931471805599453f;
 #endif
 }
 
-// Joins the parts of split work: a wave per vector, 2^(m - max m) of each
-// part's output and sum.
+// ---- few float queries over many keys ---------------------------------------------
+
+// Up to 1024 / D query vectors of a document and KV head against a range of
+// keys: the bytes of K and V bound it, and with so few queries a matrix tile
+// would be mostly empty (and three parts of every key more work than the key
+// itself). 16 lanes take a key, E = D / 16 dims each, so a wave loads four
+// keys at once straight into registers and sums a score with four lane
+// exchanges; the keys of a 16-lane group keep a softmax state of their own, and
+// groups and waves are joined at the end. A tile is 32 keys: eight per wave,
+// two per group.
+template <class T, int D, bool WHOLE>
+__global__ __launch_bounds__(256, 2) void masked_few_kernel(MaskedArgs a) {
+    constexpr int E = D / 16, NV = 1024 / D, KT = 32, KG = KT / 16;
+    __shared__ float out_s[4][NV][D];
+    __shared__ float ml_s[4][NV][2];
+    const AttnWork w = a.work[blockIdx.x];
+    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+    const int l16 = lane & 15, g = lane >> 4;
+    const int G = a.heads / a.kv_heads;
+    const int nvec = min(w.q_len * G - w.v0, NV);
+    const int shift = w.k_len - w.q_len;
+    // dims of a lane: 4 from every 64
+    float q[NV][E], o[NV][E], m[NV], l[NV], slope[NV];
+    int pos[NV], lo[NV], hi[NV];
+    auto load = [&](const T *row, float (&x)[E]) {
+#pragma unroll
+        for (int c = 0; c < E; c += 4) {
+            const int d = 16 * c + 4 * l16;
+            if constexpr (WHOLE) {
+                typename Row<T, 4>::type v = {};
+                if (d < a.hd) v = *(const typename Row<T, 4>::type *)(row + d);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[c + e] = (float)v[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[c + e] = d + e < a.hd ? (float)row[d + e] : 0.f;
+            }
+        }
+    };
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const int vec = w.v0 + min(v, nvec - 1);
+        const int qi = vec / G, head = w.kvh * G + (vec - qi * G);
+        load((const T *)a.q + (int64_t)(w.q_row + qi) * a.q_tok + head * a.q_head, q[v]);
+        const int p = qi + shift;
+        pos[v] = p;
+        lo[v] = a.window >= 0 ? (int)max((int64_t)p - a.window, (int64_t)0) : 0;
+        int64_t last = w.k_len - 1;
+        if (a.causal) last = min(last, (int64_t)p);
+        if (a.window >= 0) last = min(last, (int64_t)p + a.window);
+        hi[v] = (int)max(last, (int64_t)-1);
+        slope[v] = a.slopes ? a.slopes[head] * LOG2E : 0.f;
+        m[v] = -INFINITY;
+        l[v] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            q[v][e] *= a.scale * (a.cap > 0.f ? 1.f : LOG2E);
+            o[v][e] = 0.f;
+        }
+    }
+    const T *kbase = (const T *)a.k + w.k_row * a.k_tok + w.kvh * a.k_head;
+    const T *vbase = (const T *)a.v + w.k_row * a.v_tok + w.kvh * a.v_head;
+    const float to2x = a.cap > 0.f ? 2.f * LOG2E / a.cap : 0.f, capl = a.cap * LOG2E;
+    for (int t = w.t0; t < w.t1; ++t) {
+        const int k0 = (t < w.pre_tiles ? t * KT : w.main_key + (t - w.pre_tiles) * KT) + 4 * KG * wave + g;
+        float k[KG][E], v[KG][E], s[KG][NV];
+#pragma unroll
+        for (int i = 0; i < KG; ++i) {  // keys past the end: the last one, hidden below
+            const int64_t key = min(k0 + 4 * i, w.k_len - 1);
+            load(kbase + key * a.k_tok, k[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < KG; ++i) {
+            const int64_t key = min(k0 + 4 * i, w.k_len - 1);
+            load(vbase + key * a.v_tok, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < KG; ++i)
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                s[i][j] = -INFINITY;
+                if (j >= nvec) continue;
+                float x = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) x = __builtin_fmaf(q[j][e], k[i][e], x);
+                x = group_reduce<16, false>(x);
+                if (a.cap > 0.f) x = capped<true>(x, to2x, capl);
+                const int key = k0 + 4 * i;
+                if (a.slopes) x -= slope[j] * fabsf((float)(pos[j] - key));
+                const bool vis = key < w.k_len && (key < w.prefix || (key >= lo[j] && key <= hi[j]));
+                s[i][j] = vis ? x : -INFINITY;
+            }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            if (j >= nvec) continue;
+            float top = m[j];
+#pragma unroll
+            for (int i = 0; i < KG; ++i) top = fmaxf(top, s[i][j]);
+            const float base = top == -INFINITY ? 0.f : top;
+            const float f = __builtin_amdgcn_exp2f(m[j] - base);
+            m[j] = top;
+            l[j] *= f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[j][e] *= f;
+#pragma unroll
+            for (int i = 0; i < KG; ++i) {
+                const float p = __builtin_amdgcn_exp2f(s[i][j] - base);
+                l[j] += p;
+                // a hidden key's value may be anything
+                const bool vis = s[i][j] != -INFINITY;
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[j][e] += vis ? p * v[i][e] : 0.f;
+            }
+        }
+    }
+    // the wave's four groups, then the four waves
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const float top = group_max4(m[j]);
+        const float f = __builtin_amdgcn_exp2f(m[j] - (top == -INFINITY ? 0.f : top));
+        const float sum = group_sum4(l[j] * f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float x = group_sum4(o[j][e] * f);
+            if (g == 0) out_s[wave][j][16 * (e & ~3) + 4 * l16 + (e & 3)] = x;
+        }
+        if (lane == 0) {
+            ml_s[wave][j][0] = top;
+            ml_s[wave][j][1] = sum;
+        }
+    }
+    __syncthreads();
+    for (int j = wave; j < nvec; j += 4) {
+        float top = -INFINITY, sum = 0.f, f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, ml_s[i][j][0]);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[i] = __builtin_amdgcn_exp2f(ml_s[i][j][0] - base);
+            sum += f[i] * ml_s[i][j][1];
+        }
+        const int vec = w.v0 + j, qi = vec / G, head = w.kvh * G + (vec - qi * G);
+        const int64_t qrow = (int64_t)w.q_row + qi;
+        T *row = (T *)a.out + qrow * a.o_tok + head * a.o_head;
+        float *part = w.slot < 0 ? nullptr : a.partial + (int64_t)w.slot * (NV * (D + 2));
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) {
+            const int d = lane + 64 * e;
+            float x = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x += f[i] * out_s[i][j][d];
+            if (part) part[j * D + d] = x;
+            else if (d < a.hd) row[d] = (T)(sum == 0.f ? 0.f : x / sum);
+        }
+        if (lane == 0) {
+            if (part) {
+                part[NV * D + 2 * j] = top;
+                part[NV * D + 2 * j + 1] = sum;
+            } else if (a.lse) {
+                a.lse[qrow * a.heads + head] =
+                    sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+            }
+        }
+    }
+}
+
+// Joins the parts of split work: 2^(m - max m) of each part's output and sum.
+// A workgroup takes 32 dims of a vector. The parts' weights are found once, in
+// LDS; then eight lanes (four dims each) read a part, 32 parts at once and eight
+// rounds of them in flight: what it takes is a few dependent loads.
 template <class T>
 __global__ __launch_bounds__(256) void masked_join_kernel(MaskedArgs a, MaskedShape shape) {
+    __shared__ float f_s[MASKED_MOST_PARTS];
+    __shared__ f32x4 acc_s[4][8];
+    __shared__ float red_s[2][4];
     const AttnJoin w = a.join[blockIdx.x];
-    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int l8 = threadIdx.x & 7, group = threadIdx.x >> 3;
     const int G = a.heads / a.kv_heads;
-    const int local = blockIdx.y * 4 + wave;
-    const int vec = w.v0 + local;
-    if (local >= shape.vectors || vec >= w.q_len * G) return;
+    const int local = blockIdx.y, vec = w.v0 + local, dim = blockIdx.z * 32 + 4 * l8;
+    if (vec >= w.q_len * G) return;
     const int qi = vec / G, head = w.kvh * G + (vec - qi * G);
     const int64_t slot = (int64_t)shape.vectors * (shape.dim + 2);  // masked_slot
     const float *part = a.partial + w.slot * slot;
     const float *ml = part + shape.vectors * shape.dim + 2 * local;
-    float top = -INFINITY;
-    for (int i = lane; i < w.parts; i += 64) top = fmaxf(top, ml[i * slot]);
-    top = wave_max(top);
-    const float base = top == -INFINITY ? 0.f : top;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-    for (int i = 0; i < w.parts; ++i) {
-        const float f = __builtin_amdgcn_exp2f(ml[i * slot] - base);
-        l += f * ml[i * slot + 1];
-        const float *src = part + i * slot + local * shape.dim;
+    float m[MASKED_MOST_PARTS / 256], l[MASKED_MOST_PARTS / 256], top = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int d = lane + 64 * e;
-            if (d < a.hd) acc[e] += f * src[d];
-        }
+    for (int r = 0; r < MASKED_MOST_PARTS / 256; ++r) {
+        const int i = threadIdx.x + 256 * r;
+        m[r] = i < w.parts ? ml[i * slot] : -INFINITY;
+        l[r] = i < w.parts ? ml[i * slot + 1] : 0.f;
+        top = fmaxf(top, m[r]);
     }
+    top = wave_max(top);
+    if (lane == 0) red_s[0][wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red_s[0][0], red_s[0][1]), fmaxf(red_s[0][2], red_s[0][3]));
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < MASKED_MOST_PARTS / 256; ++r) {
+        const float f = __builtin_amdgcn_exp2f(m[r] - base);
+        f_s[threadIdx.x + 256 * r] = f;
+        sum += f * l[r];
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) red_s[1][wave] = sum;
+    __syncthreads();
+    sum = (red_s[1][0] + red_s[1][1]) + (red_s[1][2] + red_s[1][3]);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int i = group; i < w.parts; i += 32)
+        acc = acc + *(const f32x4 *)(part + i * slot + local * shape.dim + dim) * f_s[i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {  // the wave's eight groups
+        acc[e] += dpp_mov<0x128>(acc[e]);  // row_ror 8: the other half of 16 lanes
+        acc[e] = group_sum4(acc[e]);
+    }
+    if (lane < 8) acc_s[wave][l8] = acc;
+    __syncthreads();
+    if (threadIdx.x >= 8) return;
+    acc = (acc_s[0][l8] + acc_s[1][l8]) + (acc_s[2][l8] + acc_s[3][l8]);
     const int64_t qrow = (int64_t)w.q_row + qi;
     T *row = (T *)a.out + qrow * a.o_tok + head * a.o_head;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int d = lane + 64 * e;
-        if (d < a.hd) row[d] = (T)(l == 0.f ? 0.f : acc[e] / l);
-    }
-    if (a.lse && lane == 0)
+    for (int e = 0; e < 4; ++e)
+        if (dim + e < a.hd) row[dim + e] = (T)(sum == 0.f ? 0.f : acc[e] / sum);
+    if (a.lse && dim == 0)
         a.lse[qrow * a.heads + head] =
-            l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+            sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 MaskedShape masked_shape(bool bf16, int hd, int64_t most) {
-    if (hd > 256) return {0, 16, ROW_KEYS};
+    if (hd > 256) return {0, 16, ROW_KEYS, 0};
     const int dim = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
-    if (bf16) return {dim, most <= 32 ? 32 : 128, dim == 256 ? 32 : 64};
-    return {dim, 128, dim == 64 ? 64 : 32};
+    if (bf16) return {dim, most <= 32 ? 32 : 128, dim == 256 ? 32 : 64, 0};
+    if (most <= 1024 / dim) return {dim, 1024 / dim, 32, 0};
+    return {dim, 128, 32, 3};
+}
+
+template <class T, int P, int D, int KT, int WAVES, int DS, int STAGES, TileSource FROM, int MINW>
+static hipError_t launch_tiles(const MaskedArgs &a, hipStream_t s) {
+    const dim3 grid((unsigned)a.n_work), block(64 * WAVES);
+    if (a.cap > 0.f)
+        hipLaunchKernelGGL((masked_tile_kernel<T, P, D, KT, WAVES, DS, STAGES, FROM, true, MINW>),
+                           grid, block, 0, s, a);
+    else
+        hipLaunchKernelGGL((masked_tile_kernel<T, P, D, KT, WAVES, DS, STAGES, FROM, false, MINW>),
+                           grid, block, 0, s, a);
+    return hipGetLastError();
+}
+
+template <TileSource FROM>
+static hipError_t launch_bf16(const MaskedArgs &a, const MaskedShape &shape, hipStream_t s) {
+    const bool few = shape.vectors == 32;
+    switch (shape.dim) {
+        case 64:
+            return few ? launch_tiles<__bf16, 1, 64, 64, 1, 1, 2, FROM, 1>(a, s)
+                       : launch_tiles<__bf16, 1, 64, 64, 4, 1, 2, FROM, 3>(a, s);
+        case 128:
+            return few ? launch_tiles<__bf16, 1, 128, 64, 1, 1, 2, FROM, 1>(a, s)
+                       : launch_tiles<__bf16, 1, 128, 64, 4, 1, 2, FROM, 2>(a, s);
+        case 256:
+            return few ? launch_tiles<__bf16, 1, 256, 32, 1, 1, 2, FROM, 1>(a, s)
+                       : launch_tiles<__bf16, 1, 256, 32, 4, 1, 2, FROM, 2>(a, s);
+    }
+    return hipErrorInvalidValue;
+}
+
+template <bool WHOLE>
+static hipError_t launch_few(const MaskedArgs &a, const MaskedShape &shape, hipStream_t s) {
+    const dim3 grid((unsigned)a.n_work), block(256);
+    switch (shape.dim) {
+        case 64: hipLaunchKernelGGL((masked_few_kernel<float, 64, WHOLE>), grid, block, 0, s, a); break;
+        case 128: hipLaunchKernelGGL((masked_few_kernel<float, 128, WHOLE>), grid, block, 0, s, a); break;
+        default: hipLaunchKernelGGL((masked_few_kernel<float, 256, WHOLE>), grid, block, 0, s, a);
+    }
+    return hipGetLastError();
+}
+
+template <int D, int KT, int WAVES, int DS, int STAGES>
+static hipError_t launch_planes(const MaskedArgs &a, hipStream_t s) {
+    hipLaunchKernelGGL((masked_planes_kernel<D, KT>), dim3((unsigned)a.n_tiles, 2), dim3(256), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    return e != hipSuccess ? e : launch_tiles<float, 3, D, KT, WAVES, DS, STAGES, FROM_PLANES, 2>(a, s);
+}
+
+static hipError_t launch_float(const MaskedArgs &a, const MaskedShape &shape, hipStream_t s) {
+    if (shape.planes == 0) return a.whole ? launch_few<true>(a, shape, s) : launch_few<false>(a, shape, s);
+    switch (shape.dim) {
+        case 64: return launch_planes<64, 32, 4, 1, 2>(a, s);
+        case 128: return launch_planes<128, 32, 8, 2, 2>(a, s);
+        case 256: return launch_planes<256, 32, 8, 2, 1>(a, s);
+    }
+    return hipErrorInvalidValue;
 }
 
 template <class T>
@@ -685,54 +1048,22 @@ static hipError_t launch_rows(const MaskedArgs &a, int vectors, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <class T, int P, int D, int KT, int WAVES, bool WHOLE, int MINB>
-static hipError_t launch_tiles(const MaskedArgs &a, hipStream_t s) {
-    const dim3 grid((unsigned)a.n_work), block(64 * WAVES);
-    if (a.cap > 0.f) hipLaunchKernelGGL((masked_tile_kernel<T, P, D, KT, WAVES, WHOLE, true, MINB>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((masked_tile_kernel<T, P, D, KT, WAVES, WHOLE, false, MINB>), grid, block, 0, s, a);
-    return hipGetLastError();
-}
-
-template <bool WHOLE>
-static hipError_t launch_tiles_of(const MaskedArgs &a, bool bf16, const MaskedShape &shape,
-                                  hipStream_t s) {
-    if (bf16 && shape.vectors == 32) {
-        switch (shape.dim) {
-            case 64: return launch_tiles<__bf16, 1, 64, 64, 1, WHOLE, 1>(a, s);
-            case 128: return launch_tiles<__bf16, 1, 128, 64, 1, WHOLE, 1>(a, s);
-            case 256: return launch_tiles<__bf16, 1, 256, 32, 1, WHOLE, 1>(a, s);
-        }
-    } else if (bf16) {
-        switch (shape.dim) {
-            case 64: return launch_tiles<__bf16, 1, 64, 64, 4, WHOLE, 3>(a, s);
-            case 128: return launch_tiles<__bf16, 1, 128, 64, 4, WHOLE, 2>(a, s);
-            case 256: return launch_tiles<__bf16, 1, 256, 32, 4, WHOLE, 2>(a, s);
-        }
-    } else {
-        switch (shape.dim) {
-            case 64: return launch_tiles<float, 3, 64, 64, 4, WHOLE, 2>(a, s);
-            case 128: return launch_tiles<float, 3, 128, 32, 4, WHOLE, 1>(a, s);
-            case 256: return launch_tiles<float, 3, 256, 32, 4, WHOLE, 1>(a, s);
-        }
-    }
-    return hipErrorInvalidValue;
-}
-
-hipError_t launch_masked_attention(const MaskedArgs &a, bool bf16, const MaskedShape &shape,
+hipError_t launch_masked_attention(MaskedArgs a, bool bf16, const MaskedShape &shape,
                                    hipStream_t s) {
     if (a.n_work <= 0) return hipSuccess;
     if (shape.dim == 0) return bf16 ? launch_rows<__bf16>(a, shape.vectors, s)
                                     : launch_rows<float>(a, shape.vectors, s);
     // whole 16-byte chunks at 16-byte addresses
     const int64_t size = bf16 ? 2 : 4, n = 16 / size;
-    bool whole = a.hd % n == 0;
-    for (const void *p : {a.q, a.k, a.v, (const void *)a.out}) whole = whole && (uintptr_t)p % 16 == 0;
+    a.whole = a.hd % n == 0;
+    for (const void *p : {a.q, a.k, a.v, (const void *)a.out}) a.whole = a.whole && (uintptr_t)p % 16 == 0;
     for (int64_t st : {a.q_tok, a.q_head, a.k_tok, a.k_head, a.v_tok, a.v_head, a.o_tok, a.o_head})
-        whole = whole && st % n == 0;
-    const hipError_t e = whole ? launch_tiles_of<true>(a, bf16, shape, s)
-                               : launch_tiles_of<false>(a, bf16, shape, s);
+        a.whole = a.whole && st % n == 0;
+    const hipError_t e = !bf16    ? launch_float(a, shape, s)
+                         : a.whole ? launch_bf16<FROM_ROWS>(a, shape, s)
+                                   : launch_bf16<FROM_PIECES>(a, shape, s);
     if (e != hipSuccess || a.n_join == 0) return e;
-    const dim3 grid((unsigned)a.n_join, (unsigned)(shape.vectors / 4)), block(256);
+    const dim3 grid((unsigned)a.n_join, (unsigned)a.join_vectors, (unsigned)(shape.dim / 32)), block(256);
     if (bf16) hipLaunchKernelGGL(masked_join_kernel<__bf16>, grid, block, 0, s, a, shape);
     else hipLaunchKernelGGL(masked_join_kernel<float>, grid, block, 0, s, a, shape);
     return hipGetLastError();

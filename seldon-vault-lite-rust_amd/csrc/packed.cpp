@@ -104,14 +104,16 @@ struct svl_attention_plan {
     int device = 0;
     svl_attention_shape shape{};
     MaskedShape tiles{};
-    int64_t workspace = 0;
+    int64_t workspace = 0, planes_at = 0;  // bytes; planes behind the partial results
     int64_t q_rows = 0, kv_rows = 0;  // rows up to the last document's end
-    int32_t n_work = 0, n_join = 0;
+    int32_t n_work = 0, n_join = 0, join_vectors = 0, n_tiles = 0;
     AttnWork *work = nullptr;
     AttnJoin *join = nullptr;
+    AttnTiles *key_tiles = nullptr;
     ~svl_attention_plan() {
         if (work) (void)hipFree(work);
         if (join) (void)hipFree(join);
+        if (key_tiles) (void)hipFree(key_tiles);
     }
 };
 
@@ -165,9 +167,37 @@ svl_status fill_positions(svl_position_plan &plan, const svl_segment *segments, 
     return SVL_OK;
 }
 
+// The order of launch. Workgroup b runs on XCD b % 8: each takes a contiguous
+// eighth of the work, by key tiles, so that groups of one document and KV head
+// share their keys in one L2; within an XCD the longest work goes first, and
+// the short ends the launch.
+void order_work(std::vector<AttnWork> &work) {
+    constexpr int XCDS = 8;
+    auto cost = [](const AttnWork &w) { return (int64_t)(w.t1 - w.t0) + 1; };
+    int64_t total = 0;
+    for (const AttnWork &w : work) total += cost(w);
+    std::vector<AttnWork> part[XCDS];
+    int64_t before = 0;
+    for (const AttnWork &w : work) {
+        part[std::min<int64_t>(before * XCDS / total, XCDS - 1)].push_back(w);
+        before += cost(w);
+    }
+    size_t longest = 0;
+    for (auto &p : part) {
+        std::stable_sort(p.begin(), p.end(), [&](const AttnWork &a, const AttnWork &b) {
+            return cost(a) > cost(b);
+        });
+        longest = std::max(longest, p.size());
+    }
+    work.clear();
+    for (size_t i = 0; i < longest; ++i)
+        for (auto &p : part)
+            if (i < p.size()) work.push_back(p[i]);
+}
+
 svl_status fill_attention(svl_attention_plan &plan, const int64_t *qo, const int64_t *ko,
                           const int64_t *prefix, int32_t documents, std::vector<AttnWork> &work,
-                          std::vector<AttnJoin> &join) {
+                          std::vector<AttnJoin> &join, std::vector<AttnTiles> &tiles) {
     const svl_attention_shape &sh = plan.shape;
     const int64_t G = sh.num_heads / sh.num_kv_heads;
     int64_t most = 0;
@@ -179,6 +209,11 @@ svl_status fill_attention(svl_attention_plan &plan, const int64_t *qo, const int
         const int64_t ql = qo[d + 1] - qo[d], kl = ko[d + 1] - ko[d];
         const int64_t pre = prefix ? std::min(prefix[d], kl) : 0;
         const int64_t shift = kl - ql;
+        const int64_t k_tiles = (kl + KT - 1) / KT, tile0 = (int64_t)tiles.size();
+        if (plan.tiles.planes > 0 && ql > 0)
+            for (int64_t g = 0; g < sh.num_kv_heads; ++g)
+                for (int64_t t = 0; t < k_tiles; ++t)
+                    tiles.push_back({(int32_t)(ko[d] + t * KT), (int32_t)std::min(KT, kl - t * KT), (int32_t)g});
         for (int64_t g = 0; g < sh.num_kv_heads; ++g)
             for (int64_t v0 = 0; v0 < ql * G; v0 += BV) {
                 // keys that some query of the group sees: the prefix and [lo, hi]
@@ -192,21 +227,21 @@ svl_status fill_attention(svl_attention_plan &plan, const int64_t *qo, const int
                 }
                 const int64_t pre_tiles = (pre + KT - 1) / KT;
                 const int64_t first = std::max(lo / KT, pre_tiles);
-                const int64_t tiles =
+                const int64_t seen =
                     pre_tiles + (hi >= lo ? std::max<int64_t>(hi / KT + 1 - first, 0) : 0);
-                total += tiles;
+                total += seen;
                 // (keys past the last tile are never asked for, so main_key may pass them)
                 work.push_back({(int32_t)qo[d], (int32_t)ql, (int32_t)ko[d], (int32_t)kl,
                                 (int32_t)g, (int32_t)v0, (int32_t)pre, (int32_t)pre_tiles,
                                 (int32_t)std::min<int64_t>(first * KT, INT32_MAX), 0,
-                                (int32_t)tiles, -1});
+                                (int32_t)seen, -1, (int32_t)(tile0 + g * k_tiles)});
             }
     }
     // Few groups leave CUs idle: their key tiles are split over workgroups, whose
     // parts a second launch joins.
-    const int64_t target = BV == 32 ? 1280 : 512;
+    const int64_t target = BV == 32 && sh.dtype == SVL_BF16 ? MASKED_MOST_PARTS : BV < 32 ? 512 : 256;
     if (plan.tiles.dim > 0 && (int64_t)work.size() < target && total > (int64_t)work.size()) {
-        const int64_t each = std::max<int64_t>((total + target - 1) / target, 4);
+        const int64_t each = std::max<int64_t>((total + target - 1) / target, BV <= 32 ? 1 : 8);
         std::vector<AttnWork> split;
         int64_t slots = 0;
         for (const AttnWork &w : work) {
@@ -222,11 +257,17 @@ svl_status fill_attention(svl_attention_plan &plan, const int64_t *qo, const int
             if (parts > 1) slots += parts;
         }
         work.swap(split);
-        plan.workspace = slots * masked_slot(plan.tiles) * (int64_t)sizeof(float);
+        plan.planes_at = slots * masked_slot(plan.tiles) * (int64_t)sizeof(float);
     }
+    order_work(work);
     if (work.size() > INT32_MAX) return fail(SVL_LIMIT, "more than 2^31 - 1 work items");
     plan.n_work = (int32_t)work.size();
+    if (tiles.size() > INT32_MAX) return fail(SVL_LIMIT, "more than 2^31 - 1 key tiles");
+    plan.n_tiles = (int32_t)tiles.size();
+    plan.planes_at = (plan.planes_at + 15) / 16 * 16;
+    plan.workspace = plan.planes_at + plan.n_tiles * masked_tile_bytes(plan.tiles);
     plan.n_join = (int32_t)join.size();
+    plan.join_vectors = (int32_t)std::min(most, BV);
     plan.q_rows = qo[documents];
     plan.kv_rows = ko[documents];
     return SVL_OK;
@@ -386,6 +427,7 @@ svl_status svl_attention_plan_create(svl_ctx *ctx, const svl_attention_shape *sh
                                      svl_attention_plan **out) {
     std::vector<AttnWork> work;
     std::vector<AttnJoin> join;
+    std::vector<AttnTiles> tiles;
     auto build = [&](svl_attention_plan &plan) {
         if (!shape || !q_offsets) return fail(SVL_USAGE, "shape or offsets are null");
         if (documents < 0) return fail(SVL_USAGE, "document count is negative");
@@ -411,11 +453,12 @@ svl_status svl_attention_plan_create(svl_ctx *ctx, const svl_attention_shape *sh
         }
         plan.shape = *shape;
         plan.shape.window = shape->window < 0 ? -1 : std::min<int64_t>(shape->window, INT32_MAX);
-        return fill_attention(plan, q_offsets, ko, prefix, documents, work, join);
+        return fill_attention(plan, q_offsets, ko, prefix, documents, work, join, tiles);
     };
     return make_plan(ctx, out, build, [&](svl_attention_plan &plan) {
         ST_TRY(upload(work, &plan.work));
-        return upload(join, &plan.join);
+        ST_TRY(upload(join, &plan.join));
+        return upload(tiles, &plan.key_tiles);
     });
 }
 
@@ -483,7 +526,11 @@ svl_status svl_masked_attention(const svl_attention_plan *plan, const svl_attent
     a.n_work = plan->n_work;
     a.join = plan->join;
     a.n_join = plan->n_join;
+    a.join_vectors = plan->join_vectors;
     a.partial = (float *)workspace;
+    a.planes = (char *)workspace + plan->planes_at;
+    a.tiles = plan->key_tiles;
+    a.n_tiles = plan->n_tiles;
     OnDevice on(plan->device);
     HIP_TRY(on.err);
     HIP_TRY(launch_masked_attention(a, sh.dtype == SVL_BF16, plan->tiles, (hipStream_t)stream));

@@ -53,12 +53,19 @@ struct AttnWork {
     int32_t prefix;
     int32_t pre_tiles, main_key;
     int32_t t0, t1;
-    int32_t slot;  // partial result's place in the workspace, -1: to the output
+    int32_t slot;   // partial result's place in the workspace, -1: to the output
+    int32_t tile0;  // first of the document and KV head's tiles of planes
+};
+// A tile of planes: keys from row k_row on, `rows` of them.
+struct AttnTiles {
+    int32_t k_row, rows, kvh;
 };
 // A group of vectors whose key tiles were split over `parts` workgroups.
 struct AttnJoin {
     int32_t q_row, q_len, kvh, v0, slot, parts;
 };
+
+constexpr int MASKED_MOST_PARTS = 1280;  // of one group
 
 struct MaskedArgs {
     const void *q, *k, *v;
@@ -72,8 +79,12 @@ struct MaskedArgs {
     const AttnWork *work;
     int32_t n_work;
     const AttnJoin *join;
-    int32_t n_join;
+    int32_t n_join, join_vectors;  // most vectors of a joined group
     float *partial;
+    void *planes;  // float keys and values, split (null: not)
+    const AttnTiles *tiles;
+    int32_t n_tiles;
+    int32_t whole;   // every row in whole 16-byte chunks at 16-byte addresses
 };
 
 // The kernel that a plan is made for, and its tiles.
@@ -81,12 +92,17 @@ struct MaskedShape {
     int dim;      // head dim that its tiles hold, 0: the kernel of one wave a query
     int vectors;  // query vectors per workgroup
     int keys;     // keys per tile
+    int planes;   // parts that keys and values are split into before, 0: none
 };
 // most: query vectors of the batch's largest document and KV head.
 MaskedShape masked_shape(bool bf16, int hd, int64_t most);
 // Floats of a slot of the workspace: outputs, maxima and sums of its vectors.
 inline int64_t masked_slot(const MaskedShape &s) { return (int64_t)s.vectors * (s.dim + 2); }
-hipError_t launch_masked_attention(const MaskedArgs &a, bool bf16, const MaskedShape &shape,
+// Bytes of a tile of planes: keys and values.
+inline int64_t masked_tile_bytes(const MaskedShape &s) {
+    return (int64_t)2 * s.planes * s.keys * s.dim * 2;
+}
+hipError_t launch_masked_attention(MaskedArgs a, bool bf16, const MaskedShape &shape,
                                    hipStream_t s);
 
 }  // namespace svl
