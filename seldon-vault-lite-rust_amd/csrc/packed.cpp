@@ -354,11 +354,8 @@ svl_status svl_rope_axes(const svl_rope_rows *tensors, int32_t n_tensors, int32_
     a.hd = (int32_t)head_dim;
     a.pairs = (int32_t)pairs;
     const bool adjacent = layout == SVL_ROPE_ADJACENT;
-    int64_t width = dtype == SVL_BF16 ? 8 : 4;  // 16 bytes, less where something is narrower
-    auto narrow = [&](int64_t elements) {
-        while (elements % width) width /= 2;
-    };
-    narrow(pairs);
+    const int64_t size = dtype == SVL_BF16 ? 2 : 4, chunk = 16 / size;
+    bool runs = pairs % chunk == 0, rows = head_dim % chunk == 0;  // in whole chunks
     for (int64_t j = 0, run = 0; j < pairs; ++j) {
         if (pair_axis[j] >= axes)
             return fail(SVL_USAGE, "pair %lld: axis %d of %d", (long long)j, pair_axis[j], axes);
@@ -378,10 +375,9 @@ svl_status svl_rope_axes(const svl_rope_rows *tensors, int32_t n_tensors, int32_
             while (end < pairs && pair_axis[end] == pair_axis[j]) ++end;
             a.col[j] = (uint16_t)(run + j);
             a.partner[j] = (uint16_t)(end + j);
-            narrow(end - run);
+            runs = runs && (end - run) % chunk == 0;
         }
     }
-    const int64_t size = dtype == SVL_BF16 ? 2 : 4;
     bool copies = false;
     for (int i = 0; i < n_tensors; ++i) {
         const svl_rope_rows &r = tensors[i];
@@ -407,17 +403,15 @@ svl_status svl_rope_axes(const svl_rope_rows *tensors, int32_t n_tensors, int32_
         a.out_head[i] = r.out_head_stride;
         for (int64_t st : {r.heads > 1 ? r.in_head_stride : 0, r.heads > 1 ? r.out_head_stride : 0,
                            tokens > 1 ? r.in_token_stride : 0, tokens > 1 ? r.out_token_stride : 0})
-            narrow(st);
-        while (!aligned(r.in, width * size) || !aligned(r.out, width * size)) width /= 2;
+            rows = rows && st % chunk == 0;
+        rows = rows && aligned(r.in, 16) && aligned(r.out, 16);
         copies = copies || r.in != r.out;
     }
-    if (copies) {
-        a.copied = (int32_t)(head_dim - 2 * pairs);
-        narrow(a.copied);
-    }
+    if (copies) a.copied = (int32_t)(head_dim - 2 * pairs);
     if (tokens == 0 || a.heads[0] + a.heads[1] == 0 || (pairs == 0 && a.copied == 0)) return SVL_OK;
     if (pairs > 0 && !d_positions) return fail(SVL_USAGE, "positions are null");
-    HIP_TRY(launch_rope_axes(a, dtype == SVL_BF16, adjacent, (int)width, (hipStream_t)stream));
+    const RopeForm form = !rows ? ROPE_SINGLE : runs ? ROPE_CHUNKS : ROPE_ROWS;
+    HIP_TRY(launch_rope_axes(a, dtype == SVL_BF16, adjacent, form, (hipStream_t)stream));
     return SVL_OK;
 }
 

@@ -37,9 +37,11 @@ struct RopeAxesArgs {
     uint16_t partner[ROPE_MAX_PAIRS];  // its other column
     uint8_t axis[ROPE_MAX_PAIRS];
 };
-// width: pairs per unit, consecutive in both columns (adjacent: in one), and
-// every row's address a multiple of `width` elements' bytes.
-hipError_t launch_rope_axes(const RopeAxesArgs &a, bool bf16, bool adjacent, int width,
+// ROPE_CHUNKS: pairs in runs of whole 16-byte chunks in both columns (adjacent:
+// in one), every row at a multiple of 16 bytes; ROPE_ROWS: rows of whole chunks
+// at such addresses; ROPE_SINGLE: any.
+enum RopeForm { ROPE_CHUNKS, ROPE_ROWS, ROPE_SINGLE };
+hipError_t launch_rope_axes(const RopeAxesArgs &a, bool bf16, bool adjacent, RopeForm form,
                             hipStream_t s);
 
 // One workgroup's work in masked attention: query vectors v0 .. of one

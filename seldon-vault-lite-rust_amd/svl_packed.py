@@ -18,8 +18,10 @@ window (kernels.rs:1037-1135).
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import numpy as np
+import torch
 
 import svl_amd
 from svl_amd import SvlError, _check, lib
@@ -33,9 +35,9 @@ class _Segment(ctypes.Structure):
                                                  ("kind", "frames", "rows", "cols", "step")]
 
 
-class _RopeRows(ctypes.Structure):
-    _fields_ = [("inp", ctypes.c_void_p), ("out", ctypes.c_void_p)] + [
-        (n, ctypes.c_int64) for n in ("heads", "in_token", "in_head", "out_token", "out_head")]
+# svl_rope_rows of queries and of keys, and svl_attention_args, as bytes.
+_ROPE_ROWS = struct.Struct("=2Q5q")
+_ATTENTION_ARGS = struct.Struct("=5Q8q2fQ")
 
 
 class _Shape(ctypes.Structure):
@@ -44,16 +46,13 @@ class _Shape(ctypes.Structure):
                 ("causal", ctypes.c_int32), ("window", ctypes.c_int64)]
 
 
-class _Args(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "lse")] + [
-        (n, ctypes.c_int64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token",
-                                      "v_head", "out_token", "out_head")] + [
-        ("scale", ctypes.c_float), ("soft_cap", ctypes.c_float), ("slopes", ctypes.c_void_p)]
+_library = None
 
 
 def _load():
-    L = lib()
-    if not getattr(L, "_packed_ready", False):
+    global _library
+    if _library is None:
+        L = lib()
         vp, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
         L.svl_position_plan_create.argtypes = [vp, vp, i64, ctypes.POINTER(vp)]
         L.svl_position_plan_destroy.argtypes = [vp]
@@ -66,9 +65,9 @@ def _load():
         L.svl_attention_plan_destroy.argtypes = [vp]
         L.svl_attention_plan_workspace.restype = i64
         L.svl_attention_plan_workspace.argtypes = [vp]
-        L.svl_masked_attention.argtypes = [vp, ctypes.POINTER(_Args), vp, ctypes.c_size_t, vp]
-        L._packed_ready = True
-    return L
+        L.svl_masked_attention.argtypes = [vp, vp, vp, ctypes.c_size_t, vp]
+        _library = L
+    return _library
 
 
 def _usage(msg):
@@ -76,7 +75,6 @@ def _usage(msg):
 
 
 def _dtype(t):
-    import torch
     if t == torch.float32:
         return 0
     if t == torch.bfloat16:
@@ -84,34 +82,34 @@ def _dtype(t):
     raise SvlError(6, f"type {t}: float32 and bfloat16 are supported")
 
 
-def _on(device, **tensors):
-    """Every tensor given lies on the device."""
-    for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.device.index != device):
-            raise _usage(f"{name} is on {t.device}, not on cuda:{device}")
+# The calls below are a few microseconds of Python each, beside kernels of as
+# many: shapes and strides are read once, and nothing is converted that is
+# already in its form.
+
+def _on(device, name, t):
+    """The tensor lies on the device."""
+    if t.get_device() != device:
+        raise _usage(f"{name} is on {t.device}, not on cuda:{device}")
 
 
-def _rows(name, t, dtype, heads=None, head_dim=None):
-    """[tokens, heads, head dim] with a contiguous last axis."""
-    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or \
-            (head_dim is not None and t.shape[2] != head_dim):
-        raise _usage(f"{name} of shape {tuple(t.shape)}: expected [tokens, "
-                     f"{heads if heads is not None else 'heads'}, "
-                     f"{head_dim if head_dim is not None else 'head dim'}]")
+def _rows(name, t, device, dtype, tokens, heads, head_dim):
+    """[tokens, heads, head dim], at least `tokens` of them, with a contiguous
+    last axis: (data, token stride, head stride). The strides of a single token
+    or head are not used."""
+    _on(device, name, t)
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim or shape[0] < tokens:
+        raise _usage(f"{name} of shape {tuple(shape)}: expected [{tokens}, {heads}, {head_dim}]")
     if t.dtype != dtype:
         raise _usage(f"{name} is {t.dtype}, not {dtype}")
-    if t.numel() and t.shape[2] > 1 and t.stride(2) != 1:
+    token, head, last = t.stride()
+    if last != 1 and head_dim > 1 and t.numel():
         raise _usage(f"{name}: the last axis is not contiguous")
-
-
-def _strides(t):
-    """Token and head strides; those of a single token or head are not used."""
-    return [t.stride(i) if t.shape[i] > 1 else t.shape[2] for i in (0, 1)]
+    return (t.data_ptr(), token if shape[0] > 1 else head_dim, head if heads > 1 else head_dim)
 
 
 def _stream(device):
-    import torch
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _host(values, dtype):
@@ -142,18 +140,18 @@ class PositionPlan:
         self.tokens = int(_load().svl_position_plan_tokens(h))
 
     def __del__(self):
-        if getattr(self, "handle", None):
-            _load().svl_position_plan_destroy(self.handle)
+        if getattr(self, "handle", None) and _library is not None:
+            _library.svl_position_plan_destroy(self.handle)
             self.handle = None
 
 
 def axis_positions(plan: PositionPlan, out):
     """Positions of the plan's tokens into `out` [tokens, 3] (int32)."""
-    import torch
-    _on(plan.device.ordinal, out=out)
-    if out.dtype != torch.int32 or tuple(out.shape) != (plan.tokens, 3) or not out.is_contiguous():
+    device = plan.device.ordinal
+    _on(device, "out", out)
+    if out.dtype != torch.int32 or out.shape != (plan.tokens, 3) or not out.is_contiguous():
         raise _usage(f"positions of {plan.tokens} tokens take a contiguous int32 [tokens, 3]")
-    _check(_load().svl_axis_positions(plan.handle, svl_amd._dp(out), _stream(out.device)))
+    _check(_load().svl_axis_positions(plan.handle, out.data_ptr(), _stream(device)))
 
 
 def rope_axes(q, k, positions, inv_freq, pair_axis, layout, out_q, out_k):
@@ -161,11 +159,12 @@ def rope_axes(q, k, positions, inv_freq, pair_axis, layout, out_q, out_k):
     [tokens, axes] (int32): pair j by positions[:, pair_axis[j]] *
     inv_freq[j], its columns by `layout` (ROPE_LAYOUTS). out_q and out_k may
     be q and k."""
-    import torch
     if layout not in ROPE_LAYOUTS:
         raise _usage(f"rotation layout {layout!r} is not one of {sorted(ROPE_LAYOUTS)}")
-    device = q.device.index
-    _on(device, q=q, k=k, positions=positions, out_q=out_q, out_k=out_k)
+    if q.dim() != 3 or not q.is_cuda:
+        raise _usage("q must be [tokens, heads, head dim] on a GPU")
+    device, dtype = q.get_device(), q.dtype
+    _on(device, "positions", positions)
     if positions.dim() != 2 or positions.dtype != torch.int32 or not positions.is_contiguous():
         raise _usage("positions must be a contiguous int32 [tokens, axes]")
     tokens, axes = positions.shape
@@ -174,26 +173,28 @@ def rope_axes(q, k, positions, inv_freq, pair_axis, layout, out_q, out_k):
         raise _usage("one frequency and one axis per pair are required")
     if (k is None) != (out_k is None):
         raise _usage("keys and their output come together")
-    if q.dim() != 3:
-        raise _usage("q must be [tokens, heads, head dim]")
-    hd = q.shape[2]
-    rows = (_RopeRows * 2)()
-    n = 0
+    code, hd = _dtype(dtype), q.shape[2]
+    rows, n = b"", 0
     for name, x, y in (("q", q, out_q), ("k", k, out_k)):
         if x is None:
             continue
-        _rows(name, x, q.dtype, None, hd)
-        _rows(f"out_{name}", y, q.dtype, x.shape[1], hd)
+        heads = x.shape[1]
+        data, token, head = _rows(name, x, device, dtype, tokens, heads, hd)
+        out, out_token, out_head = _rows(f"out_{name}", y, device, dtype, tokens, heads, hd)
         if x.shape[0] != tokens or y.shape[0] != tokens:
-            raise _usage(f"{name} has {x.shape[0]} tokens, positions {tokens}, "
-                         f"its output {y.shape[0]}")
-        rows[n] = _RopeRows(x.data_ptr(), y.data_ptr(), x.shape[1], *_strides(x),
-                            *_strides(y))
+            raise _usage(f"{name} and its output have {x.shape[0]} and {y.shape[0]} tokens, "
+                         f"positions {tokens}")
+        rows += _ROPE_ROWS.pack(data, out, heads, token, head, out_token, out_head)
         n += 1
-    with torch.cuda.device(device):
-        _check(_load().svl_rope_axes(rows, n, _dtype(q.dtype), svl_amd._dp(positions), tokens,
-                                     axes, hd, _array(freq), _array(axis), freq.size,
-                                     ROPE_LAYOUTS[layout], _stream(device)))
+    # bytes pass as pointers that live as long as the call
+    call = (rows, n, code, positions.data_ptr(), tokens, axes, hd, freq.tobytes(), axis.tobytes(),
+            freq.size, ROPE_LAYOUTS[layout], _stream(device))
+    if torch.cuda.current_device() == device:
+        status = _load().svl_rope_axes(*call)
+    else:
+        with torch.cuda.device(device):
+            status = _load().svl_rope_axes(*call)
+    _check(status)
 
 
 class AttentionPlan:
@@ -227,8 +228,8 @@ class AttentionPlan:
         self.workspace_bytes = int(_load().svl_attention_plan_workspace(h))
 
     def __del__(self):
-        if getattr(self, "handle", None):
-            _load().svl_attention_plan_destroy(self.handle)
+        if getattr(self, "handle", None) and _library is not None:
+            _library.svl_attention_plan_destroy(self.handle)
             self.handle = None
 
 
@@ -240,31 +241,36 @@ def masked_attention(plan: AttentionPlan, q, k, v, out, scale, soft_cap=0.0, slo
     rows, heads] float32 receives the log of each row's sum. Rows outside
     every document are left as they were. workspace: at least
     plan.workspace_bytes of uint8, or None to allocate it for the call."""
-    import torch
-    device = plan.device.ordinal
-    _on(device, q=q, k=k, v=v, out=out, slopes=slopes, lse=lse, workspace=workspace)
+    device, dtype = plan.device.ordinal, plan.dtype
     nh, kv, hd = plan.num_heads, plan.num_kv_heads, plan.head_dim
-    for name, t, heads, least in (("q", q, nh, plan.q_rows), ("k", k, kv, plan.kv_rows),
-                                  ("v", v, kv, plan.kv_rows), ("out", out, nh, plan.q_rows)):
-        _rows(name, t, plan.dtype, heads, hd)
-        if t.shape[0] < least:
-            raise _usage(f"{name} has {t.shape[0]} rows, the plan {least}")
-    if slopes is not None and (slopes.dtype != torch.float32 or tuple(slopes.shape) != (nh,) or
-                               not slopes.is_contiguous()):
-        raise _usage(f"slopes must be a contiguous float32 [{nh}]")
-    if lse is not None and (lse.dtype != torch.float32 or lse.dim() != 2 or
-                            lse.shape[0] < plan.q_rows or lse.shape[1] != nh or
-                            not lse.is_contiguous()):
-        raise _usage(f"lse must be a contiguous float32 [query rows, {nh}]")
-    if workspace is None:
-        if plan.workspace_bytes:
-            workspace = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=q.device)
-    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-        raise _usage("the workspace must be a contiguous uint8 tensor")
-    args = _Args(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                 None if lse is None else lse.data_ptr(), *_strides(q), *_strides(k),
-                 *_strides(v), *_strides(out),
-                 float(scale), float(soft_cap), None if slopes is None else slopes.data_ptr())
-    _check(_load().svl_masked_attention(
-        plan.handle, ctypes.byref(args), svl_amd._dp(workspace),
-        0 if workspace is None else workspace.numel(), _stream(q.device)))
+    rows = [_rows("q", q, device, dtype, plan.q_rows, nh, hd),
+            _rows("k", k, device, dtype, plan.kv_rows, kv, hd),
+            _rows("v", v, device, dtype, plan.kv_rows, kv, hd),
+            _rows("out", out, device, dtype, plan.q_rows, nh, hd)]
+    lse_ptr = slope_ptr = 0
+    work_ptr, size = None, 0
+    if slopes is not None:
+        _on(device, "slopes", slopes)
+        if slopes.dtype != torch.float32 or slopes.shape != (nh,) or not slopes.is_contiguous():
+            raise _usage(f"slopes must be a contiguous float32 [{nh}]")
+        slope_ptr = slopes.data_ptr()
+    if lse is not None:
+        _on(device, "lse", lse)
+        if lse.dtype != torch.float32 or lse.dim() != 2 or lse.shape[0] < plan.q_rows or \
+                lse.shape[1] != nh or not lse.is_contiguous():
+            raise _usage(f"lse must be a contiguous float32 [query rows, {nh}]")
+        lse_ptr = lse.data_ptr()
+    if workspace is None and plan.workspace_bytes:
+        workspace = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=q.device)
+    if workspace is not None:
+        _on(device, "workspace", workspace)
+        if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+            raise _usage("the workspace must be a contiguous uint8 tensor")
+        work_ptr, size = workspace.data_ptr(), workspace.numel()
+    (qp, *qs), (kp, *ks), (vp, *vs), (op, *os) = rows
+    try:
+        args = _ATTENTION_ARGS.pack(qp, kp, vp, op, lse_ptr, *qs, *ks, *vs, *os, scale, soft_cap,
+                                    slope_ptr)
+    except (OverflowError, struct.error):
+        raise _usage(f"scale {scale} or cap {soft_cap} is no 32-bit number") from None
+    _check(_load().svl_masked_attention(plan.handle, args, work_ptr, size, _stream(device)))

@@ -118,8 +118,18 @@ def test_rotation(tokens, heads, kv, hd, pairs, layout, order, dtype):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("layout", ["half", "adjacent", "axial"])
-def test_rotation_in_place(layout, dtype):
-    check_rope(np.random.default_rng(4), 77, 3, 1, 64, 24, layout, "runs", dtype, inplace=True)
+@pytest.mark.parametrize("hd,pairs", [(64, 24), (64, 30), (37, 7), (256, 128)])
+def test_rotation_in_place(hd, pairs, layout, dtype):
+    check_rope(np.random.default_rng(4), 77, 3, 1, hd, pairs, layout, "runs", dtype, inplace=True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("heads,kv,hd,pairs", [(64, 8, 256, 120), (40, 40, 128, 64), (3, 3, 1024, 250),
+                                               (70, 0, 33, 16)])
+def test_rotation_of_many_heads(heads, kv, hd, pairs, dtype):
+    """More values a token than a workgroup's threads hold at once."""
+    for layout in ("half", "axial"):
+        check_rope(np.random.default_rng(7), 9, heads, kv, hd, pairs, layout, "runs", dtype)
 
 
 @pytest.mark.parametrize("far", [10**6, 2**31 - 4000, -2**31 + 100])

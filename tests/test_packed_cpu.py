@@ -59,7 +59,8 @@ def _rope(tokens=4, axes=2, hd=8, pairs=4, layout=0, dtype=0, n=1, freq=None, ax
     L = P._load()
     r = dict(inp=1024, out=4096, heads=2, in_token=16, in_head=8, out_token=16, out_head=8)
     r.update(row)
-    rows = (P._RopeRows * 1)(P._RopeRows(**r))
+    rows = P._ROPE_ROWS.pack(*[r[k] or 0 for k in ("inp", "out", "heads", "in_token", "in_head",
+                                                   "out_token", "out_head")])
     freq = np.ones(max(pairs, 1), np.float32) if freq is None else freq
     axis = np.zeros(max(pairs, 1), np.uint8) if axis is None else axis
     return L.svl_rope_axes(rows, n, dtype, positions, tokens, axes, hd, P._array(freq),
