@@ -336,8 +336,9 @@ __device__ __forceinline__ float capped(float s, float to2x, float capl) {
 //  * O^T += V^T P^T: the score registers 8 u .. 8 u + 7 are the B operand of
 //    step u as they stand (keys 16 u + 4 h + 0..3 and + 8, h = lane / 32), and V
 //    is read transposed in the same order.
-//  * The running maximum moves only when a query's grows by more than 2^8, so
-//    outputs are rarely rescaled.
+//  * The running maximum moves only when some query's weights of a tile add up
+//    to more than MOST_SUM, so outputs are rarely rescaled and most tiles look
+//    for no maximum at all.
 //  * STAGES = 2: a tile's K and V come in under the whole tile before, one
 //    barrier a tile. STAGES = 1, where LDS holds no more: V(t) comes in under
 //    the scores of tile t, K(t + 1) under its softmax and P V; two barriers.
@@ -346,12 +347,14 @@ __device__ __forceinline__ float capped(float s, float to2x, float capl) {
 //    SIMD to a single wave (float rows: three parts of every query; 256 dims
 //    311 us with one wave, 214 us with two).
 // P = 1: bfloat16 operands; weights are rounded to bfloat16 for the product
-// with V (a relative 2^-8 of each, the output's own step); their sum is taken
-// before, so that the lse keeps its 32 bits.
+// with V (a relative 2^-8 of each, the output's own step). LSE: their sum is
+// taken before, so that the lse keeps its 32 bits, else of the rounded ones.
 // P = 3: float operands as three bfloat16 parts; of the nine products the six
 // above 2^-24 are taken, the five small ones in an accumulator of their own.
+constexpr float MOST_SUM = 16384.f;
+
 template <class T, int P, int D, int KT, int WAVES, int DS, int STAGES, TileSource FROM, bool CAP,
-          int MINW>
+          bool LSE, int MINW>
 __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int DW = D / DS;  // dims of a wave
@@ -386,7 +389,8 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
         if (a.window >= 0) k = min(k, (int64_t)pos + a.window);
         return (int)max(k, (int64_t)-1);
     };
-    const int lo = first_key(p), hi = last_key(p);
+    const int lo = first_key(p);
+    const uint32_t span = (uint32_t)max(last_key(p) - lo + 1, 0);  // keys from lo on
     // the wave's: any of its queries, all of them; and all of the workgroup's
     const int any_lo = first_key(p_lo), any_hi = last_key(p_hi);
     const int all_lo = first_key(p_hi), all_hi = last_key(p_lo);
@@ -463,15 +467,16 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
         vc.fetch(FROM == FROM_PLANES ? vbase + (int64_t)k0 * (2 * P * D) : vbase + (int64_t)k0 * ldv,
                  ldv, a.hd, min(KT, w.k_len - k0), to);
     };
-    // Lane addresses, in elements: K row l32 of a block at chunk h, V row
+    // Lane addresses, in bytes: K row l32 of a block at chunk h, V row
     // (lane % 16) / 4 of four at its chunk of a 32-dim tile. Rows start at
     // multiples of D, so another chunk (a multiple of 2 or 4 further before the
     // swizzle) is an exclusive or of the offset; it is done as each fragment is
     // read (kept in registers, the addresses would spill).
-    int koff = l32 * D + (((dim0 / 8 + h) ^ key_swizzle<D>(l32)) << 3);
+    int koff = l32 * D * 2 + (((dim0 / 8 + h) ^ key_swizzle<D>(l32)) << 4);
     const int vr = 4 * h + ((lane & 15) >> 2);
-    int voff = vr * D + (((dim0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ value_swizzle<D>(vr)) << 3) +
-               4 * (lane & 1);
+    int voff = vr * D * 2 +
+               (((dim0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ value_swizzle<D>(vr)) << 4) +
+               8 * (lane & 1);
 
     f32x16 s[NK];
     auto scores = [&](const __bf16 *Ks) {
@@ -482,7 +487,7 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
             for (int r = 0; r < 16; ++r) big[r] = rest[r] = 0.f;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const __bf16 *at = Ks + (koff ^ (16 * b));
+                const __bf16 *at = (const __bf16 *)((const char *)Ks + (koff ^ (32 * b)));
                 bf16x8 k[P];
 #pragma unroll
                 for (int i = 0; i < P; ++i) k[i] = *(const bf16x8 *)(at + i * KT * D + kb * 32 * D);
@@ -521,7 +526,7 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
                     for (int e = 0; e < 4; ++e) s[kb][r + e] += x[e];
                 }
         }
-        float tmax = -INFINITY, mul = to_log2;
+        float mul = to_log2;
         if (CAP || a.slopes || !all) {  // to log2 units first
             mul = 1.f;
 #pragma unroll
@@ -543,58 +548,78 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
                 for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int key = k0 + 32 * kb + 8 * (r >> 2) + 4 * h + (r & 3);
-                        s[kb][r] = key < w.prefix || (key >= lo && key <= hi) ? s[kb][r] : -INFINITY;
+                        // key - lo as an unsigned number is at most hi - lo inside
+                        const int key = k0 + 4 * h + 32 * kb + 8 * (r >> 2) + (r & 3);
+                        const bool vis = (key < w.prefix) | ((uint32_t)(key - lo) < span);
+                        s[kb][r] = vis ? s[kb][r] : -INFINITY;
                     }
             }
         }
+        bf16x8 pr[P][NK][2];
+        auto exponentials = [&]() {  // the weights, and this lane's sum of them
+            const float base = m_ref == -INFINITY ? 0.f : -m_ref;
+            float psum = 0.f;
 #pragma unroll
-        for (int kb = 0; kb < NK; ++kb)
+            for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[kb][r]);
-        tmax = other_half_max(tmax) * mul;
-        const bool grow = tmax > m_ref + 8.f;
-        if (__ballot(grow)) {
-            const float m_new = grow ? tmax : m_ref;
+                for (int u = 0; u < 2; ++u) {
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * u + i], mul, base));
+                        if constexpr (LSE || P == 3) psum += e[i];
+                    }
+                    if constexpr (P == 1) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) pr[0][kb][u][i] = (__bf16)e[i];
+                        if constexpr (!LSE) {
+#pragma unroll
+                            for (int i = 0; i < 8; i += 2)
+                                psum = __builtin_amdgcn_fdot2_f32_bf16(
+                                    bf16x2{pr[0][kb][u][i], pr[0][kb][u][i + 1]},
+                                    bf16x2{(__bf16)1.f, (__bf16)1.f}, psum, false);
+                        }
+                    } else {
+                        u32x4 pl[P];
+#pragma unroll
+                        for (int i = 0; i < 8; i += 2) {
+                            uint32_t x[3];
+                            split3<true>(e[i], e[i + 1], x);
+#pragma unroll
+                            for (int j = 0; j < P; ++j) pl[j][i / 2] = x[j];
+                        }
+#pragma unroll
+                        for (int j = 0; j < P; ++j) pr[j][kb][u] = __builtin_bit_cast(bf16x8, pl[j]);
+                    }
+                }
+            return psum;
+        };
+        // With the maximum of before, where there is one: weights that have not
+        // grown too large need no new one.
+        bool renew = __ballot(m_ref == -INFINITY) != 0;
+        float psum = 0.f;
+        if (!renew) {
+            psum = exponentials();
+            renew = __ballot(!(psum <= MOST_SUM)) != 0;
+        }
+        if (renew) {
+            float tmax = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[kb][r]);
+            const float m_new = fmaxf(m_ref, other_half_max(tmax) * mul);
             const float alpha = m_ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref - m_new);
             l_run *= alpha;
 #pragma unroll
             for (int d = 0; d < NT; ++d) o[d] = o[d] * alpha;
             m_ref = m_new;
+            psum = exponentials();
         }
-        const float base = m_ref == -INFINITY ? 0.f : -m_ref;
-        bf16x8 pr[P][NK][2];
-        float psum = 0.f;
-#pragma unroll
-        for (int kb = 0; kb < NK; ++kb)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float e[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * u + i], mul, base));
-                    psum += e[i];
-                }
-                if constexpr (P == 1) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) pr[0][kb][u][i] = (__bf16)e[i];
-                } else {
-                    u32x4 pl[P];
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        uint32_t x[3];
-                        split3<true>(e[i], e[i + 1], x);
-#pragma unroll
-                        for (int j = 0; j < P; ++j) pl[j][i / 2] = x[j];
-                    }
-#pragma unroll
-                    for (int j = 0; j < P; ++j) pr[j][kb][u] = __builtin_bit_cast(bf16x8, pl[j]);
-                }
-            }
-        l_run += other_half_sum(psum);
+        l_run += psum;
 #pragma unroll
         for (int d = 0; d < NT; ++d) {
-            const __bf16 *tile = Vs + (voff ^ (32 * d));
+            const __bf16 *tile = (const __bf16 *)((const char *)Vs + (voff ^ (64 * d)));
             f32x16 rest;
             if constexpr (P == 3) {
 #pragma unroll
@@ -696,6 +721,7 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
         }
     }
 
+    l_run = other_half_sum(l_run);
     float *part = w.slot < 0 ? nullptr : a.partial + (int64_t)w.slot * (VECTORS * (D + 2));
     if (redo) {
         for (int i = wave; i < VECTORS && w.v0 + i < nvec; i += WAVES)
@@ -718,6 +744,12 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
         }
         return;
     }
+    if (l_run == 0.f) {  // nothing seen (or scores of -inf alone, whose 0 * v may be NaN)
+#pragma unroll
+        for (int d = 0; d < NT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    }
     const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
     const int64_t qrow = (int64_t)w.q_row + qi;
     T *row = (T *)a.out + qrow * a.o_tok + head * a.o_head;
@@ -728,7 +760,7 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
             const int dim = dim0 + 32 * d + 2 * r + 4 * h;
             typename Row<T, 4>::type y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = (T)(l_run == 0.f ? 0.f : o[d][r + e] * inv);
+            for (int e = 0; e < 4; ++e) y[e] = (T)(o[d][r + e] * inv);
             if (a.whole) {
                 if (dim < a.hd) *(typename Row<T, 4>::type *)(row + dim) = y;
             } else {
@@ -979,21 +1011,33 @@ __global__ __launch_bounds__(256) void masked_join_kernel(MaskedArgs a, MaskedSh
 MaskedShape masked_shape(bool bf16, int hd, int64_t most) {
     if (hd > 256) return {0, 16, ROW_KEYS, 0};
     const int dim = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
-    if (bf16) return {dim, most <= 32 ? 32 : 128, dim == 256 ? 32 : 64, 0};
+    if (bf16) return {dim, most <= 32 ? 32 : 128, dim == 256 || (dim == 128 && most > 32) ? 32 : 64, 0};
     if (most <= 1024 / dim) return {dim, 1024 / dim, 32, 0};
     return {dim, 128, 32, 3};
 }
 
-template <class T, int P, int D, int KT, int WAVES, int DS, int STAGES, TileSource FROM, int MINW>
-static hipError_t launch_tiles(const MaskedArgs &a, hipStream_t s) {
+template <class T, int P, int D, int KT, int WAVES, int DS, int STAGES, TileSource FROM, int MINW,
+          bool CAP>
+static hipError_t launch_tiles_capped(const MaskedArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)a.n_work), block(64 * WAVES);
-    if (a.cap > 0.f)
-        hipLaunchKernelGGL((masked_tile_kernel<T, P, D, KT, WAVES, DS, STAGES, FROM, true, MINW>),
+    // The sum of rounded weights costs half as much and is what the rounded
+    // products are to be divided by, but no lse; it is worth a kernel of its own
+    // where vector work bounds it (video 1197 -> 1168 us), not where keys' bytes do.
+    constexpr bool ROUNDED = P == 1 && WAVES > 1 && FROM == FROM_ROWS;
+    if (ROUNDED && !a.lse)
+        hipLaunchKernelGGL((masked_tile_kernel<T, P, D, KT, WAVES, DS, STAGES, FROM, CAP, !ROUNDED, MINW>),
                            grid, block, 0, s, a);
     else
-        hipLaunchKernelGGL((masked_tile_kernel<T, P, D, KT, WAVES, DS, STAGES, FROM, false, MINW>),
+        hipLaunchKernelGGL((masked_tile_kernel<T, P, D, KT, WAVES, DS, STAGES, FROM, CAP, true, MINW>),
                            grid, block, 0, s, a);
     return hipGetLastError();
+}
+
+template <class T, int P, int D, int KT, int WAVES, int DS, int STAGES, TileSource FROM, int MINW>
+static hipError_t launch_tiles(const MaskedArgs &a, hipStream_t s) {
+    return a.cap > 0.f
+               ? launch_tiles_capped<T, P, D, KT, WAVES, DS, STAGES, FROM, MINW, true>(a, s)
+               : launch_tiles_capped<T, P, D, KT, WAVES, DS, STAGES, FROM, MINW, false>(a, s);
 }
 
 template <TileSource FROM>
@@ -1002,10 +1046,10 @@ static hipError_t launch_bf16(const MaskedArgs &a, const MaskedShape &shape, hip
     switch (shape.dim) {
         case 64:
             return few ? launch_tiles<__bf16, 1, 64, 64, 1, 1, 2, FROM, 1>(a, s)
-                       : launch_tiles<__bf16, 1, 64, 64, 4, 1, 2, FROM, 3>(a, s);
+                       : launch_tiles<__bf16, 1, 64, 64, 4, 1, 2, FROM, 4>(a, s);
         case 128:
             return few ? launch_tiles<__bf16, 1, 128, 64, 1, 1, 2, FROM, 1>(a, s)
-                       : launch_tiles<__bf16, 1, 128, 64, 4, 1, 2, FROM, 2>(a, s);
+                       : launch_tiles<__bf16, 1, 128, 32, 4, 1, 2, FROM, 3>(a, s);
         case 256:
             return few ? launch_tiles<__bf16, 1, 256, 32, 1, 1, 2, FROM, 1>(a, s)
                        : launch_tiles<__bf16, 1, 256, 32, 4, 1, 2, FROM, 2>(a, s);

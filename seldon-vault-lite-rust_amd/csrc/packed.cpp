@@ -5,6 +5,7 @@
 #include <climits>
 #include <memory>
 #include <new>
+#include <numeric>
 
 #include "host_common.hpp"
 #include "packed.hpp"
@@ -167,32 +168,61 @@ svl_status fill_positions(svl_position_plan &plan, const svl_segment *segments, 
     return SVL_OK;
 }
 
-// The order of launch. Workgroup b runs on XCD b % 8: each takes a contiguous
-// eighth of the work, by key tiles, so that groups of one document and KV head
-// share their keys in one L2; within an XCD the longest work goes first, and
-// the short ends the launch.
+// The order of launch. Workgroup b runs on XCD b % 8, and the groups of one
+// document and KV head (beside each other in `work`) share their keys in its L2:
+// whole ones go to the XCD with the least work, longest first, large ones in
+// pieces of half an XCD's share. A piece takes its groups at a stride of the
+// golden ratio, so that each has the short and the long ones of a causal mask;
+// an XCD whose groups are all long would run a second round for a few of them
+// (64 documents of 64-512 tokens: contiguous eighths 191 us, this order
+// ORDER_US). Within an XCD the longest go first, and the short ones end the
+// launch.
 void order_work(std::vector<AttnWork> &work) {
-    constexpr int XCDS = 8;
-    auto cost = [](const AttnWork &w) { return (int64_t)(w.t1 - w.t0) + 1; };
+    constexpr size_t XCDS = 8;
+    auto cost = [](const AttnWork &w) { return (int64_t)(w.t1 - w.t0) + 2; };  // 2: start and end
+    auto longer = [&](const AttnWork &a, const AttnWork &b) { return cost(a) > cost(b); };
     int64_t total = 0;
     for (const AttnWork &w : work) total += cost(w);
-    std::vector<AttnWork> part[XCDS];
-    int64_t before = 0;
-    for (const AttnWork &w : work) {
-        part[std::min<int64_t>(before * XCDS / total, XCDS - 1)].push_back(w);
-        before += cost(w);
+    struct Piece {
+        std::vector<AttnWork> work;
+        int64_t cost = 0;
+    };
+    std::vector<Piece> pieces;
+    for (size_t i = 0; i < work.size();) {
+        size_t n = 1;
+        while (i + n < work.size() && work[i + n].q_row == work[i].q_row &&
+               work[i + n].kvh == work[i].kvh)
+            ++n;
+        size_t stride = std::max<size_t>((size_t)((double)n * 0.618), 1);
+        while (std::gcd(stride, n) > 1) ++stride;
+        pieces.emplace_back();
+        for (size_t k = 0; k < n; ++k) {
+            if (pieces.back().cost * 2 * (int64_t)XCDS >= total) pieces.emplace_back();
+            const AttnWork &w = work[i + k * stride % n];
+            pieces.back().work.push_back(w);
+            pieces.back().cost += cost(w);
+        }
+        i += n;
+    }
+    std::stable_sort(pieces.begin(), pieces.end(),
+                     [](const Piece &a, const Piece &b) { return a.cost > b.cost; });
+    Piece part[XCDS];
+    for (Piece &p : pieces) {
+        Piece *least = std::min_element(part, part + XCDS, [](const Piece &a, const Piece &b) {
+            return a.cost < b.cost;
+        });
+        least->work.insert(least->work.end(), p.work.begin(), p.work.end());
+        least->cost += p.cost;
     }
     size_t longest = 0;
-    for (auto &p : part) {
-        std::stable_sort(p.begin(), p.end(), [&](const AttnWork &a, const AttnWork &b) {
-            return cost(a) > cost(b);
-        });
-        longest = std::max(longest, p.size());
+    for (Piece &p : part) {
+        std::stable_sort(p.work.begin(), p.work.end(), longer);
+        longest = std::max(longest, p.work.size());
     }
     work.clear();
     for (size_t i = 0; i < longest; ++i)
-        for (auto &p : part)
-            if (i < p.size()) work.push_back(p[i]);
+        for (const Piece &p : part)
+            if (i < p.work.size()) work.push_back(p.work[i]);
 }
 
 svl_status fill_attention(svl_attention_plan &plan, const int64_t *qo, const int64_t *ko,

@@ -257,7 +257,7 @@ template <class T, int R>
 __global__ __launch_bounds__(256) void rope_rows_kernel(RopeAxesArgs a, int heads_each) {
     constexpr int C = 16 / sizeof(T);
     typedef typename Row<T, C>::type Chunk;
-    extern __shared__ char lds[];
+    extern __shared__ char rope_s[];
     const int chunks = a.hd / C;                   // of a head row
     const int heads = a.heads[0] + a.heads[1];
     const int h0 = blockIdx.y * heads_each, here = min(heads_each, heads - h0);
@@ -272,11 +272,11 @@ __global__ __launch_bounds__(256) void rope_rows_kernel(RopeAxesArgs a, int head
     // a token's part of LDS: the heads' rows, a chunk of zeros, the turns
     const int zero_at = chunks * heads_each * 16, turns_at = zero_at + 16;
     const int each = turns_at + a.hd * 8, step = many * R;
-    char *mine_s = lds + group * R * each;         // of the first buffer
+    char *mine_s = rope_s + group * R * each;         // of the first buffer
     // partners' bytes from the token's part
     int partner[C];
     {
-        int *of = (int *)lds;
+        int *of = (int *)rope_s;
         for (int c = threadIdx.x; c < a.hd; c += 256) of[c] = -1;
         __syncthreads();
         for (int j = threadIdx.x; j < a.pairs; j += 256) {
@@ -291,10 +291,10 @@ __global__ __launch_bounds__(256) void rope_rows_kernel(RopeAxesArgs a, int head
         }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < 2 * step; i += 256) *(f32x4 *)(lds + i * each + zero_at) = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = threadIdx.x; i < 2 * step; i += 256) *(f32x4 *)(rope_s + i * each + zero_at) = f32x4{0.f, 0.f, 0.f, 0.f};
     const int rest = a.hd - 2 * a.pairs;           // columns without a turn
     for (int i = threadIdx.x; i < 2 * step * rest; i += 256)
-        *(float2 *)(lds + i / rest * each + turns_at + (2 * a.pairs + i % rest) * 8) =
+        *(float2 *)(rope_s + i / rest * each + turns_at + (2 * a.pairs + i % rest) * 8) =
             make_float2(1.f, -0.f);
     int buffer = 0;
     for (int64_t t0 = (int64_t)blockIdx.x * step; t0 < a.tokens; t0 += (int64_t)gridDim.x * step) {

@@ -346,7 +346,7 @@ def test_attention_keys_of_one_row():
 @pytest.mark.parametrize("dtype", TYPES)
 def test_attention_scores_past_the_range_of_exponentials(dtype):
     """Scores of +-10^5: one key takes all the weight, v p / p. p need not be one (a kernel may keep
-    a maximum up to 2^8 behind), so the result is not v to the bit: in 32 bits the product of three
+    a maximum some powers of two behind), so the result is not v to the bit: in 32 bits the product of three
     parts by three rounds at each of its six sums and leaves out 2 half steps, 1 / p is off by up
     to 2 and the last product by one, 12 in all; in bfloat16 p and the result are rounded to it."""
     rng = np.random.default_rng(11)
