@@ -229,46 +229,46 @@ struct TileCopy {
     }
 };
 
-// Float keys and values as planes: three bfloat16 parts of a tile of KT keys of
-// a document and KV head, each in the order of LDS, keys and dims past the end
-// zero. Done once a call: splitting them in every workgroup that reads them was
-// a third of the vector work of the tile kernel (documents of 64-512 tokens, 3
-// heads of 256: 214 us against FLOAT_US).
-template <int D, int KT>
+// Keys and values as tiles of KT rows in the order of LDS, keys and dims past the
+// end zero: float ones in three planes, one for each bfloat16 part, and bfloat16
+// ones of head dims that are no whole chunks. Done once a call: splitting floats
+// in every workgroup that reads them was a third of the vector work of the tile
+// kernel (64 documents of 64-512 tokens, 3 heads of 256: 214 us against 181 + 17),
+// and rows of 100 bfloat16 values read one by one took 1296 us for
+// ODD_US (4 x 4096 tokens, 8 heads).
+template <class T, int P, int D, int KT>
 __global__ __launch_bounds__(256) void masked_planes_kernel(MaskedArgs a) {
     const AttnTiles w = a.tiles[blockIdx.x];
     const bool values = blockIdx.y != 0;
-    const float *base = (const float *)(values ? a.v : a.k) +
-                        (int64_t)w.k_row * (values ? a.v_tok : a.k_tok) +
-                        w.kvh * (values ? a.v_head : a.k_head);
     const int64_t ld = values ? a.v_tok : a.k_tok;
-    __bf16 *out = (__bf16 *)a.planes + ((int64_t)blockIdx.x * 2 + values) * (3 * KT * D);
+    const T *base = (const T *)(values ? a.v : a.k) + (int64_t)w.k_row * ld +
+                    w.kvh * (values ? a.v_head : a.k_head);
+    __bf16 *out = (__bf16 *)a.planes + ((int64_t)blockIdx.x * 2 + values) * (P * KT * D);
     for (int c = threadIdx.x; c < KT * D / 8; c += 256) {
         const int r = c / (D / 8);
         const int dim = 8 * ((c % (D / 8)) ^ (values ? value_swizzle<D>(r) : key_swizzle<D>(r)));
-        float x[8];
-        const float *row = base + r * ld + dim;
-        if (r < w.rows && a.whole && dim + 8 <= a.hd) {
-            const f32x4 u = *(const f32x4 *)row, v = *(const f32x4 *)(row + 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = u[e];
-                x[4 + e] = v[e];
-            }
+        T x[8];
+        const T *row = base + r * ld + dim;
+        if (P == 3 && r < w.rows && a.whole && dim + 8 <= a.hd) {
+            __builtin_memcpy(x, __builtin_assume_aligned(row, 16), sizeof x);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = r < w.rows && dim + e < a.hd ? row[e] : 0.f;
+            for (int e = 0; e < 8; ++e) x[e] = r < w.rows && dim + e < a.hd ? row[e] : (T)0.f;
         }
-        u32x4 pl[3];
+        u32x4 pl[P];
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-            uint32_t y[3];
-            split3<false>(x[e], x[e + 1], y);
+            if constexpr (P == 1) {
+                pl[0][e / 2] = __builtin_bit_cast(uint32_t, bf16x2{x[e], x[e + 1]});
+            } else {
+                uint32_t y[3];
+                split3<false>(x[e], x[e + 1], y);
 #pragma unroll
-            for (int p = 0; p < 3; ++p) pl[p][e / 2] = y[p];
+                for (int p = 0; p < P; ++p) pl[p][e / 2] = y[p];
+            }
         }
 #pragma unroll
-        for (int p = 0; p < 3; ++p) *(u32x4 *)(out + p * KT * D + c * 8) = pl[p];
+        for (int p = 0; p < P; ++p) *(u32x4 *)(out + p * KT * D + c * 8) = pl[p];
     }
 }
 
@@ -775,19 +775,23 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
 #endif
 }
 
+// Keys of a tile of the kernel of few queries.
+constexpr int few_keys(int dim) { return 8192 / dim; }
+constexpr int FEW_PARTS = 8;
+
 // ---- few float queries over many keys ---------------------------------------------
 
-// Up to 1024 / D query vectors of a document and KV head against a range of
+// Up to NV query vectors of a document and KV head against a range of
 // keys: the bytes of K and V bound it, and with so few queries a matrix tile
 // would be mostly empty (and three parts of every key more work than the key
 // itself). 16 lanes take a key, E = D / 16 dims each, so a wave loads four
 // keys at once straight into registers and sums a score with four lane
 // exchanges; the keys of a 16-lane group keep a softmax state of their own, and
-// groups and waves are joined at the end. A tile is 32 keys: eight per wave,
-// two per group.
-template <class T, int D, bool WHOLE>
+// groups and waves are joined at the end. A group's keys of a tile, two of 256
+// dims, four of 128 or eight of 64, are loaded together.
+template <class T, int D, int NV, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void masked_few_kernel(MaskedArgs a) {
-    constexpr int E = D / 16, NV = 1024 / D, KT = 32, KG = KT / 16;
+    constexpr int E = D / 16, KT = few_keys(D), KG = KT / 16;
     __shared__ float out_s[4][NV][D];
     __shared__ float ml_s[4][NV][2];
     const AttnWork w = a.work[blockIdx.x];
@@ -1008,12 +1012,68 @@ __global__ __launch_bounds__(256) void masked_join_kernel(MaskedArgs a, MaskedSh
             sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
+// The same for at most FEW_PARTS parts of many vectors: D / 4 lanes take a
+// vector's dims and go over the parts.
+template <class T>
+__global__ __launch_bounds__(256) void masked_join_few_kernel(MaskedArgs a, MaskedShape shape) {
+    const AttnJoin w = a.join[blockIdx.x];
+    const int lanes = shape.dim / 4, each = 256 / lanes;
+    const int local = blockIdx.y * each + (int)threadIdx.x / lanes, vec = w.v0 + local;
+    const int dim = (int)threadIdx.x % lanes * 4;
+    const int G = a.heads / a.kv_heads;
+    if (local >= shape.vectors || vec >= w.q_len * G) return;
+    const int qi = vec / G, head = w.kvh * G + (vec - qi * G);
+    const int64_t slot = (int64_t)shape.vectors * (shape.dim + 2);  // masked_slot
+    const float *part = a.partial + w.slot * slot;
+    const float *ml = part + shape.vectors * shape.dim + 2 * local;
+    float m[FEW_PARTS], l[FEW_PARTS], top = -INFINITY, sum = 0.f;
+    f32x4 x[FEW_PARTS], acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < FEW_PARTS; ++i) {
+        const bool in = i < w.parts;
+        m[i] = in ? ml[i * slot] : -INFINITY;
+        l[i] = in ? ml[i * slot + 1] : 0.f;
+        x[i] = in ? *(const f32x4 *)(part + i * slot + local * shape.dim + dim) : acc;
+        top = fmaxf(top, m[i]);
+    }
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int i = 0; i < FEW_PARTS; ++i) {
+        const float f = __builtin_amdgcn_exp2f(m[i] - base);
+        sum += f * l[i];
+        acc = acc + x[i] * f;
+    }
+    const int64_t qrow = (int64_t)w.q_row + qi;
+    T *row = (T *)a.out + qrow * a.o_tok + head * a.o_head;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (dim + e < a.hd) row[dim + e] = (T)(sum == 0.f ? 0.f : acc[e] / sum);
+    if (a.lse && dim == 0)
+        a.lse[qrow * a.heads + head] =
+            sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+}
+
+// What a batch is run by:
+//  * head dims above 256: a wave a query.
+//  * up to few_vectors float queries of a document and KV head: straight from
+//    registers (a matrix tile of them took 756 us for 200003 keys, 82 this way);
+//    bfloat16 ones are as fast as the bytes on the matrix cores, 32 to a
+//    workgroup of one wave (4 queries of 128 dims over 2000-8192 keys of 64
+//    requests: 128 us, 358 from registers, where the vector work is the bound).
+//  * else 128 queries to a workgroup. Tiles of 32 keys leave room for a third
+//    workgroup a CU at 128 dims (prefix mask 1139 -> 1111 us), of 64 for a
+//    fourth at 64 dims (1264 us with tiles of 32, 1137).
 MaskedShape masked_shape(bool bf16, int hd, int64_t most) {
-    if (hd > 256) return {0, 16, ROW_KEYS, 0};
+    if (hd > 256) return {0, 16, ROW_KEYS, 0, 2048, 16};
     const int dim = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
-    if (bf16) return {dim, most <= 32 ? 32 : 128, dim == 256 || (dim == 128 && most > 32) ? 32 : 64, 0};
-    if (most <= 1024 / dim) return {dim, 1024 / dim, 32, 0};
-    return {dim, 128, 32, 3};
+    if (bf16) {
+        const int planes = hd % 8 ? 1 : 0;
+        if (most <= 32) return {dim, 32, dim == 256 ? 32 : 64, planes, 1280, 1};
+        return {dim, 128, dim == 64 ? 64 : 32, planes, dim == 64 ? 1024 : dim == 128 ? 768 : 512, 8};
+    }
+    const int few = dim == 256 ? 4 : 8;
+    if (most <= few) return {dim, most <= 1 ? 1 : most <= 4 ? 4 : 8, few_keys(dim), 0, 512, 1};
+    return {dim, 128, 32, 3, dim == 64 ? 512 : 256, 8};
 }
 
 template <class T, int P, int D, int KT, int WAVES, int DS, int STAGES, TileSource FROM, int MINW,
@@ -1057,30 +1117,55 @@ static hipError_t launch_bf16(const MaskedArgs &a, const MaskedShape &shape, hip
     return hipErrorInvalidValue;
 }
 
-template <bool WHOLE>
-static hipError_t launch_few(const MaskedArgs &a, const MaskedShape &shape, hipStream_t s) {
+template <int D, int NV>
+static hipError_t launch_few(const MaskedArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)a.n_work), block(256);
-    switch (shape.dim) {
-        case 64: hipLaunchKernelGGL((masked_few_kernel<float, 64, WHOLE>), grid, block, 0, s, a); break;
-        case 128: hipLaunchKernelGGL((masked_few_kernel<float, 128, WHOLE>), grid, block, 0, s, a); break;
-        default: hipLaunchKernelGGL((masked_few_kernel<float, 256, WHOLE>), grid, block, 0, s, a);
-    }
+    if (a.whole) hipLaunchKernelGGL((masked_few_kernel<float, D, NV, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((masked_few_kernel<float, D, NV, false>), grid, block, 0, s, a);
     return hipGetLastError();
 }
 
-template <int D, int KT, int WAVES, int DS, int STAGES>
+template <class T, int P, int D, int KT>
 static hipError_t launch_planes(const MaskedArgs &a, hipStream_t s) {
-    hipLaunchKernelGGL((masked_planes_kernel<D, KT>), dim3((unsigned)a.n_tiles, 2), dim3(256), 0, s, a);
-    const hipError_t e = hipGetLastError();
-    return e != hipSuccess ? e : launch_tiles<float, 3, D, KT, WAVES, DS, STAGES, FROM_PLANES, 2>(a, s);
+    if (a.n_tiles > 0)
+        hipLaunchKernelGGL((masked_planes_kernel<T, P, D, KT>), dim3((unsigned)a.n_tiles, 2), dim3(256),
+                           0, s, a);
+    return hipGetLastError();
 }
 
 static hipError_t launch_float(const MaskedArgs &a, const MaskedShape &shape, hipStream_t s) {
-    if (shape.planes == 0) return a.whole ? launch_few<true>(a, shape, s) : launch_few<false>(a, shape, s);
+    if (shape.planes == 0) switch (shape.dim * 16 + shape.vectors) {
+        case 64 * 16 + 1: return launch_few<64, 1>(a, s);
+        case 64 * 16 + 4: return launch_few<64, 4>(a, s);
+        case 64 * 16 + 8: return launch_few<64, 8>(a, s);
+        case 128 * 16 + 1: return launch_few<128, 1>(a, s);
+        case 128 * 16 + 4: return launch_few<128, 4>(a, s);
+        case 128 * 16 + 8: return launch_few<128, 8>(a, s);
+        case 256 * 16 + 1: return launch_few<256, 1>(a, s);
+        case 256 * 16 + 4: return launch_few<256, 4>(a, s);
+        default: return hipErrorInvalidValue;
+    }
     switch (shape.dim) {
-        case 64: return launch_planes<64, 32, 4, 1, 2>(a, s);
-        case 128: return launch_planes<128, 32, 8, 2, 2>(a, s);
-        case 256: return launch_planes<256, 32, 8, 2, 1>(a, s);
+        case 64: return launch_tiles<float, 3, 64, 32, 4, 1, 2, FROM_PLANES, 2>(a, s);
+        case 128: return launch_tiles<float, 3, 128, 32, 8, 2, 2, FROM_PLANES, 2>(a, s);
+        case 256: return launch_tiles<float, 3, 256, 32, 8, 2, 1, FROM_PLANES, 2>(a, s);
+    }
+    return hipErrorInvalidValue;
+}
+
+static hipError_t launch_planes_of(const MaskedArgs &a, bool bf16, const MaskedShape &shape,
+                                   hipStream_t s) {
+    if (!bf16) switch (shape.dim) {
+        case 64: return launch_planes<float, 3, 64, 32>(a, s);
+        case 128: return launch_planes<float, 3, 128, 32>(a, s);
+        case 256: return launch_planes<float, 3, 256, 32>(a, s);
+        default: return hipErrorInvalidValue;
+    }
+    switch (shape.dim * 64 + shape.keys) {
+        case 64 * 64 + 64: return launch_planes<__bf16, 1, 64, 64>(a, s);
+        case 128 * 64 + 64: return launch_planes<__bf16, 1, 128, 64>(a, s);
+        case 128 * 64 + 32: return launch_planes<__bf16, 1, 128, 32>(a, s);
+        case 256 * 64 + 32: return launch_planes<__bf16, 1, 256, 32>(a, s);
     }
     return hipErrorInvalidValue;
 }
@@ -1103,13 +1188,26 @@ hipError_t launch_masked_attention(MaskedArgs a, bool bf16, const MaskedShape &s
     for (const void *p : {a.q, a.k, a.v, (const void *)a.out}) a.whole = a.whole && (uintptr_t)p % 16 == 0;
     for (int64_t st : {a.q_tok, a.q_head, a.k_tok, a.k_head, a.v_tok, a.v_head, a.o_tok, a.o_head})
         a.whole = a.whole && st % n == 0;
-    const hipError_t e = !bf16    ? launch_float(a, shape, s)
-                         : a.whole ? launch_bf16<FROM_ROWS>(a, shape, s)
-                                   : launch_bf16<FROM_PIECES>(a, shape, s);
+    hipError_t e = shape.planes > 0 ? launch_planes_of(a, bf16, shape, s) : hipSuccess;
+    if (e != hipSuccess) return e;
+    e = !bf16             ? launch_float(a, shape, s)
+        : shape.planes > 0 ? launch_bf16<FROM_PLANES>(a, shape, s)
+        : a.whole          ? launch_bf16<FROM_ROWS>(a, shape, s)
+                           : launch_bf16<FROM_PIECES>(a, shape, s);
     if (e != hipSuccess || a.n_join == 0) return e;
-    const dim3 grid((unsigned)a.n_join, (unsigned)a.join_vectors, (unsigned)(shape.dim / 32)), block(256);
-    if (bf16) hipLaunchKernelGGL(masked_join_kernel<__bf16>, grid, block, 0, s, a, shape);
-    else hipLaunchKernelGGL(masked_join_kernel<float>, grid, block, 0, s, a, shape);
+    const unsigned joins = (unsigned)a.n_join, vectors = (unsigned)a.join_vectors;
+    // (16 parts of one query in the other kernel: 4.5 us, 5.5 here; 4 parts of 128: 3 us here,
+    // 80 there)
+    if (a.join_parts <= FEW_PARTS) {
+        const unsigned each = 1024u / (unsigned)shape.dim;
+        const dim3 grid(joins, (vectors + each - 1) / each), block(256);
+        if (bf16) hipLaunchKernelGGL(masked_join_few_kernel<__bf16>, grid, block, 0, s, a, shape);
+        else hipLaunchKernelGGL(masked_join_few_kernel<float>, grid, block, 0, s, a, shape);
+    } else {
+        const dim3 grid(joins, vectors, (unsigned)(shape.dim / 32)), block(256);
+        if (bf16) hipLaunchKernelGGL(masked_join_kernel<__bf16>, grid, block, 0, s, a, shape);
+        else hipLaunchKernelGGL(masked_join_kernel<float>, grid, block, 0, s, a, shape);
+    }
     return hipGetLastError();
 }
 

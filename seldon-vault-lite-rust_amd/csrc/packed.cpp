@@ -107,7 +107,7 @@ struct svl_attention_plan {
     MaskedShape tiles{};
     int64_t workspace = 0, planes_at = 0;  // bytes; planes behind the partial results
     int64_t q_rows = 0, kv_rows = 0;  // rows up to the last document's end
-    int32_t n_work = 0, n_join = 0, join_vectors = 0, n_tiles = 0;
+    int32_t n_work = 0, n_join = 0, join_vectors = 0, join_parts = 0, n_tiles = 0;
     AttnWork *work = nullptr;
     AttnJoin *join = nullptr;
     AttnTiles *key_tiles = nullptr;
@@ -267,27 +267,30 @@ svl_status fill_attention(svl_attention_plan &plan, const int64_t *qo, const int
                                 (int32_t)seen, -1, (int32_t)(tile0 + g * k_tiles)});
             }
     }
-    // Few groups leave CUs idle: their key tiles are split over workgroups, whose
-    // parts a second launch joins.
-    const int64_t target = BV == 32 && sh.dtype == SVL_BF16 ? MASKED_MOST_PARTS : BV < 32 ? 512 : 256;
-    if (plan.tiles.dim > 0 && (int64_t)work.size() < target && total > (int64_t)work.size()) {
-        const int64_t each = std::max<int64_t>((total + target - 1) / target, BV <= 32 ? 1 : 8);
+    // Groups that leave slots empty, or that are longer than half again the share of
+    // one, are split over workgroups, whose parts a second launch joins.
+    const int64_t slots = plan.tiles.slots;
+    if (plan.tiles.dim > 0 && 4 * (int64_t)work.size() < 3 * slots) {
+        const int64_t each = std::max<int64_t>((total + slots - 1) / slots, plan.tiles.least);
         std::vector<AttnWork> split;
-        int64_t slots = 0;
+        int64_t used = 0;
         for (const AttnWork &w : work) {
-            const int64_t parts = std::max<int64_t>((w.t1 + each - 1) / each, 1);
-            if (parts > 1) join.push_back({w.q_row, w.q_len, w.kvh, w.v0, (int32_t)slots, (int32_t)parts});
+            const int64_t parts = 2 * w.t1 > 3 * each ? (w.t1 + each - 1) / each : 1;
+            if (parts > 1) {
+                join.push_back({w.q_row, w.q_len, w.kvh, w.v0, (int32_t)used, (int32_t)parts});
+                plan.join_parts = std::max(plan.join_parts, (int32_t)parts);
+            }
             for (int64_t i = 0; i < parts; ++i) {
                 AttnWork x = w;
                 x.t0 = (int32_t)(w.t1 * i / parts);
                 x.t1 = (int32_t)(w.t1 * (i + 1) / parts);
-                x.slot = parts > 1 ? (int32_t)(slots + i) : -1;
+                x.slot = parts > 1 ? (int32_t)(used + i) : -1;
                 split.push_back(x);
             }
-            if (parts > 1) slots += parts;
+            if (parts > 1) used += parts;
         }
         work.swap(split);
-        plan.planes_at = slots * masked_slot(plan.tiles) * (int64_t)sizeof(float);
+        plan.planes_at = used * masked_slot(plan.tiles) * (int64_t)sizeof(float);
     }
     order_work(work);
     if (work.size() > INT32_MAX) return fail(SVL_LIMIT, "more than 2^31 - 1 work items");
@@ -551,6 +554,7 @@ svl_status svl_masked_attention(const svl_attention_plan *plan, const svl_attent
     a.join = plan->join;
     a.n_join = plan->n_join;
     a.join_vectors = plan->join_vectors;
+    a.join_parts = plan->join_parts;
     a.partial = (float *)workspace;
     a.planes = (char *)workspace + plan->planes_at;
     a.tiles = plan->key_tiles;

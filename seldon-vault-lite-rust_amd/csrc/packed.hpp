@@ -81,9 +81,9 @@ struct MaskedArgs {
     const AttnWork *work;
     int32_t n_work;
     const AttnJoin *join;
-    int32_t n_join, join_vectors;  // most vectors of a joined group
+    int32_t n_join, join_vectors, join_parts;  // most vectors and parts of a joined group
     float *partial;
-    void *planes;  // float keys and values, split (null: not)
+    void *planes;  // tiles of keys and values, where the shape has them
     const AttnTiles *tiles;
     int32_t n_tiles;
     int32_t whole;   // every row in whole 16-byte chunks at 16-byte addresses
@@ -95,6 +95,8 @@ struct MaskedShape {
     int vectors;  // query vectors per workgroup
     int keys;     // keys per tile
     int planes;   // parts that keys and values are split into before, 0: none
+    int slots;    // workgroups that the GPU holds at once
+    int least;    // key tiles that are worth a workgroup of their own
 };
 // most: query vectors of the batch's largest document and KV head.
 MaskedShape masked_shape(bool bf16, int hd, int64_t most);
