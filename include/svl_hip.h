@@ -651,8 +651,8 @@ typedef struct {
 /* Positions start at 0 in each document. A text run at p takes
  * (p + i, p + i, p + i) and moves p by its length; a grid at p takes
  * (p + step * frame, p + row, p + col) and moves p past its largest extent,
- * max(step * (frames - 1) + 1, rows, cols). At most 2^31 - 1 tokens, positions
- * below 2^31 -> LIMIT. */
+ * max(step * (frames - 1) + 1, rows, cols). More than 2^31 - 4096 tokens, or a
+ * position of 2^31 -> LIMIT. */
 svl_status svl_position_plan_create(svl_ctx *ctx, const svl_segment *segments, int64_t n,
                                     svl_position_plan **out);
 svl_status svl_position_plan_destroy(svl_position_plan *plan);
@@ -682,7 +682,7 @@ typedef struct {
  * fraction), in 32 bits, rounded once; columns from 2 * pairs on are copied.
  * One or two tensors (queries and keys) in one launch. dtype SVL_F32 or
  * SVL_BF16; 1..4 axes; inv_freq and pair_axis [pairs] on the host; head_dim at
- * most 1024, pairs at most 256. Rows of `out` must not overlap others of `in`.
+ * most 1024, pairs at most 256, heads at most 32767. Rows of `out` must not overlap others of `in`.
  * Runs on the current device. */
 svl_status svl_rope_axes(const svl_rope_rows *tensors, int32_t n_tensors, int32_t dtype,
                          const int32_t *d_positions, int64_t tokens, int32_t axes,
@@ -706,7 +706,8 @@ typedef struct {
  * be none. A key j is visible to a query of its document at position p if it
  * is one of the first prefix[d] keys (NULL: none), or if
  * (not causal or j <= p) and (no window or |p - j| <= window). Offsets start
- * at 0 or later and do not decrease; at most 2^31 - 1 rows. */
+ * at 0 or later and do not decrease. More than 2^31 - 4096 rows, or groups of
+ * queries (32 or 128 a KV head) or key tiles past 2^23 - 1 -> LIMIT. */
 svl_status svl_attention_plan_create(svl_ctx *ctx, const svl_attention_shape *shape,
                                      const int64_t *q_offsets, const int64_t *kv_offsets,
                                      const int64_t *prefix, int32_t documents,

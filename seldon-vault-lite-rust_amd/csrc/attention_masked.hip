@@ -439,7 +439,7 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
         }
     }
     const float to_log2 = size * LOG2E;
-    const float to2x = CAP ? 2.f * LOG2E * size / a.cap : 0.f, capl = a.cap * LOG2E;
+    const float to2x = CAP ? fminf(2.f * LOG2E * size / a.cap, 3e38f) : 0.f, capl = a.cap * LOG2E;
     const float slope = a.slopes ? a.slopes[head] * LOG2E : 0.f;
 
     f32x16 o[NT];
@@ -651,6 +651,7 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
     };
 
     if (threadIdx.x == 0) dirty = 0;
+    __syncthreads();
     bool redo = false;
     // V(t) has landed in the thread's part: whether values that are hidden from
     // some of the workgroup's queries are finite. They must not reach those
@@ -841,7 +842,7 @@ __global__ __launch_bounds__(256, 2) void masked_few_kernel(MaskedArgs a) {
     }
     const T *kbase = (const T *)a.k + w.k_row * a.k_tok + w.kvh * a.k_head;
     const T *vbase = (const T *)a.v + w.k_row * a.v_tok + w.kvh * a.v_head;
-    const float to2x = a.cap > 0.f ? 2.f * LOG2E / a.cap : 0.f, capl = a.cap * LOG2E;
+    const float to2x = a.cap > 0.f ? fminf(2.f * LOG2E / a.cap, 3e38f) : 0.f, capl = a.cap * LOG2E;
     for (int t = w.t0; t < w.t1; ++t) {
         const int k0 = (t < w.pre_tiles ? t * KT : w.main_key + (t - w.pre_tiles) * KT) + 4 * KG * wave + g;
         float k[KG][E], v[KG][E], s[KG][NV];

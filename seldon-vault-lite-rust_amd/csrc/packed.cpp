@@ -66,6 +66,9 @@ svl_status make_plan(svl_ctx *ctx, P **out, Build &&build, Bring &&bring) {
 
 bool aligned(const void *p, int64_t bytes) { return (uintptr_t)p % (uintptr_t)bytes == 0; }
 
+// Rows and tokens: a tile past the last one still has 32-bit indexes. Workgroups:
+// a launch counts its threads in 32 bits.
+constexpr int64_t MAX_ROWS = INT32_MAX - 4095, MAX_WORKGROUPS = (INT64_C(1) << 23) - 1;
 // Largest strides in elements: a row's offset then stays below 2^57 bytes, and
 // a tile of 64 rows within 31 bits.
 constexpr int64_t MAX_TOKEN_STRIDE = INT64_C(1) << 22, MAX_HEAD_STRIDE = INT64_C(1) << 40;
@@ -149,8 +152,7 @@ svl_status fill_positions(svl_position_plan &plan, const svl_segment *segments, 
         if (count == 0) continue;
         if (at + extent > INT32_MAX)
             return fail(SVL_LIMIT, "segment %lld: a position reaches 2^31", (long long)i);
-        if (tokens + count > INT32_MAX)
-            return fail(SVL_LIMIT, "more than 2^31 - 1 tokens");
+        if (tokens + count > MAX_ROWS) return fail(SVL_LIMIT, "more than 2^31 - 4096 tokens");
         PositionSegment d{(int32_t)tokens, (int32_t)at, 0, 1, 0};
         if (grid) {
             d.area = s.rows * s.cols;
@@ -234,6 +236,14 @@ svl_status fill_attention(svl_attention_plan &plan, const int64_t *qo, const int
     for (int32_t d = 0; d < documents; ++d) most = std::max(most, (qo[d + 1] - qo[d]) * G);
     plan.tiles = masked_shape(sh.dtype == SVL_BF16, (int)sh.head_dim, most);
     const int64_t KT = plan.tiles.keys, BV = plan.tiles.vectors;
+    int64_t groups = 0, key_tiles = 0;
+    for (int32_t d = 0; d < documents; ++d) {
+        const int64_t ql = qo[d + 1] - qo[d];
+        groups += (ql * G + BV - 1) / BV * sh.num_kv_heads;
+        if (ql > 0) key_tiles += (ko[d + 1] - ko[d] + KT - 1) / KT * sh.num_kv_heads;
+        if (groups > MAX_WORKGROUPS || (plan.tiles.planes > 0 && key_tiles > MAX_WORKGROUPS))
+            return fail(SVL_LIMIT, "more than 2^23 - 1 groups of queries or tiles of keys");
+    }
     int64_t total = 0;  // key tiles of all groups
     for (int32_t d = 0; d < documents; ++d) {
         const int64_t ql = qo[d + 1] - qo[d], kl = ko[d + 1] - ko[d];
@@ -299,9 +309,7 @@ svl_status fill_attention(svl_attention_plan &plan, const int64_t *qo, const int
         plan.planes_at = used * masked_slot(plan.tiles) * (int64_t)sizeof(float);
     }
     order_work(work);
-    if (work.size() > INT32_MAX) return fail(SVL_LIMIT, "more than 2^31 - 1 work items");
     plan.n_work = (int32_t)work.size();
-    if (tiles.size() > INT32_MAX) return fail(SVL_LIMIT, "more than 2^31 - 1 key tiles");
     plan.n_tiles = (int32_t)tiles.size();
     plan.planes_at = (plan.planes_at + 15) / 16 * 16;
     plan.workspace = plan.planes_at + plan.n_tiles * masked_tile_bytes(plan.tiles);
@@ -317,7 +325,7 @@ svl_status check_offsets(const int64_t *off, int32_t documents, const char *what
     for (int32_t d = 0; d < documents; ++d)
         if (off[d + 1] < off[d])
             return fail(SVL_USAGE, "%s offset %d decreases", what, d + 1);
-    if (off[documents] > INT32_MAX) return fail(SVL_LIMIT, "more than 2^31 - 1 %s rows", what);
+    if (off[documents] > MAX_ROWS) return fail(SVL_LIMIT, "more than 2^31 - 4096 %s rows", what);
     return SVL_OK;
 }
 
@@ -385,7 +393,7 @@ svl_status svl_rope_axes(const svl_rope_rows *tensors, int32_t n_tensors, int32_
     if (pairs > 0 && (!inv_freq || !pair_axis))
         return fail(SVL_USAGE, "frequencies or axes of the pairs are null");
     if (tokens < 0) return fail(SVL_USAGE, "token count is negative");
-    if (tokens > INT32_MAX) return fail(SVL_LIMIT, "more than 2^31 - 1 tokens");
+    if (tokens > MAX_ROWS) return fail(SVL_LIMIT, "more than 2^31 - 4096 tokens");
     RopeAxesArgs a{};
     a.pos = d_positions;
     a.tokens = tokens;
@@ -421,7 +429,7 @@ svl_status svl_rope_axes(const svl_rope_rows *tensors, int32_t n_tensors, int32_
     for (int i = 0; i < n_tensors; ++i) {
         const svl_rope_rows &r = tensors[i];
         if (r.heads < 0) return fail(SVL_USAGE, "head count is negative");
-        if (r.heads > 65536) return fail(SVL_LIMIT, "more than 65536 heads");
+        if (r.heads > 32767) return fail(SVL_LIMIT, "more than 32767 heads");
         if (r.heads == 0 || tokens == 0) continue;
         if (!r.in || !r.out) return fail(SVL_USAGE, "rows are null");
         ST_TRY(check_strides(r.in_token_stride, r.in_head_stride));
@@ -449,6 +457,7 @@ svl_status svl_rope_axes(const svl_rope_rows *tensors, int32_t n_tensors, int32_
     if (copies) a.copied = (int32_t)(head_dim - 2 * pairs);
     if (tokens == 0 || a.heads[0] + a.heads[1] == 0 || (pairs == 0 && a.copied == 0)) return SVL_OK;
     if (pairs > 0 && !d_positions) return fail(SVL_USAGE, "positions are null");
+    if (!aligned(d_positions, 4)) return fail(SVL_USAGE, "positions are not aligned to 4 bytes");
     const RopeForm form = !rows ? ROPE_SINGLE : runs ? ROPE_CHUNKS : ROPE_ROWS;
     HIP_TRY(launch_rope_axes(a, dtype == SVL_BF16, adjacent, form, (hipStream_t)stream));
     return SVL_OK;

@@ -254,14 +254,14 @@ static hipError_t launch_rope_width(const RopeAxesArgs &a, bool adjacent, hipStr
 // pairs, 92 with one token in flight); where runs are longer the units are as
 // fast and start sooner (17 tokens, 4 heads of 256: 4.7 us, 7.3 by rows).
 template <class T, int R>
-__global__ __launch_bounds__(256) void rope_rows_kernel(RopeAxesArgs a, int heads_each) {
+__global__ __launch_bounds__(256) void rope_rows_kernel(RopeAxesArgs a, int heads_each, int many) {
     constexpr int C = 16 / sizeof(T);
     typedef typename Row<T, C>::type Chunk;
     extern __shared__ char rope_s[];
     const int chunks = a.hd / C;                   // of a head row
     const int heads = a.heads[0] + a.heads[1];
     const int h0 = blockIdx.y * heads_each, here = min(heads_each, heads - h0);
-    const int used = chunks * here, many = 256 / (chunks * heads_each);  // tokens side by side
+    const int used = chunks * here;                // threads a token, `many` tokens side by side
     const int group = (int)threadIdx.x / used, lane = (int)threadIdx.x - group * used;
     const bool mine = group < many;
     const int hh = h0 + lane / chunks, col = (lane % chunks) * C;
@@ -342,12 +342,14 @@ __global__ __launch_bounds__(256) void rope_rows_kernel(RopeAxesArgs a, int head
 template <class T, int R>
 static hipError_t launch_rope_rows(const RopeAxesArgs &a, hipStream_t s) {
     const int chunks = a.hd * (int)sizeof(T) / 16, heads = a.heads[0] + a.heads[1];
-    const int each = std::min(heads, 256 / chunks), many = 256 / (chunks * each);
+    const int each = std::min(heads, 256 / chunks);
+    const int part = chunks * each * 16 + 16 + a.hd * 8;  // LDS a token: at most 12 KB
+    const int many = std::min(256 / (chunks * each), std::max(48 * 1024 / (2 * R * part), 1));
     const int64_t rounds = (a.tokens + many * R - 1) / (many * R);
     const int groups = (heads + each - 1) / each;
     const dim3 grid((unsigned)std::min<int64_t>(rounds, std::max(8192 / groups, 1)), (unsigned)groups);
-    const size_t lds = (size_t)2 * R * many * (chunks * each * 16 + 16 + a.hd * 8);
-    hipLaunchKernelGGL((rope_rows_kernel<T, R>), grid, dim3(256), lds, s, a, each);
+    const size_t lds = (size_t)2 * R * many * part;
+    hipLaunchKernelGGL((rope_rows_kernel<T, R>), grid, dim3(256), lds, s, a, each, many);
     return hipGetLastError();
 }
 

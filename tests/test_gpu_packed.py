@@ -110,7 +110,7 @@ def check_rope(rng, tokens, heads, kv, hd, pairs, layout, order, dtype, far=0, i
 @pytest.mark.parametrize("tokens,heads,kv,hd,pairs", [
     (1, 1, 1, 2, 1), (5, 3, 1, 256, 128), (301, 12, 12, 64, 30), (64, 4, 2, 128, 32),
     (3, 2, 0, 37, 18), (130, 1, 1, 48, 24), (2, 5, 5, 512, 256), (9, 2, 2, 26, 9),
-    (4, 3, 1, 64, 0)])
+    (4, 3, 1, 64, 0), (700, 1, 0, 64, 30), (1000, 1, 0, 8, 3), (3, 1, 1, 1024, 255)])
 def test_rotation(tokens, heads, kv, hd, pairs, layout, order, dtype):
     check_rope(np.random.default_rng(tokens + hd), tokens, heads, kv, hd, pairs, layout, order,
                dtype)
@@ -268,11 +268,28 @@ def test_attention_later_part_of_a_prompt(mask, dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("extra", [dict(cap=50.0, gain=8.0), dict(cap=5.0, gain=8.0),
                                    dict(slopes=True), dict(cap=20.0, slopes=True, causal=True),
-                                   dict(scale=-0.1), dict(scale=0.0), dict(cap=0.01),
+                                   dict(scale=-0.1), dict(scale=0.0), dict(cap=0.01), dict(cap=1e-39),
                                    dict(cap=1e4, gain=20.0)])
 @pytest.mark.parametrize("nh,nkv,hd", HEADS)
 def test_attention_cap_and_bias(nh, nkv, hd, extra, dtype):
     check_attention(4, [200, 1, 77], [200, 900, 130], nh, nkv, hd, dtype, **extra)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nh,nkv,hd", [(1, 1, 64), (5, 1, 64), (8, 1, 128), (1, 1, 128), (1, 1, 256),
+                                       (9, 1, 128), (40, 1, 64), (6, 3, 100), (3, 1, 250)])
+def test_attention_single_queries_by_their_count(nh, nkv, hd, dtype):
+    """One query of one to forty heads a KV head, over keys split many and few ways."""
+    check_attention(15, [1, 1, 1], [9000, 3, 400], nh, nkv, hd, dtype, causal=True, slopes=nh > 4,
+                    cap=30.0 if hd == 128 else 0.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 1, 128), (3, 1, 256), (2, 2, 64), (2, 1, 100)])
+def test_attention_few_long_prompts(nh, nkv, hd, dtype):
+    """Few groups of many queries, whose keys are split."""
+    check_attention(16, [70, 33], [3500, 2000], nh, nkv, hd, dtype, causal=True,
+                    prefix=[100, 0], window=None if hd == 64 else 1500)
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -76,7 +76,7 @@ def _rope(tokens=4, axes=2, hd=8, pairs=4, layout=0, dtype=0, n=1, freq=None, ax
     (dict(axis=np.array([0, 1, 2, 0], np.uint8)), U),
     (dict(freq=np.array([1, np.inf, 1, 1], np.float32)), U),
     (dict(freq=np.array([1, np.nan, 1, 1], np.float32)), U),
-    (dict(heads=-1), U), (dict(heads=65537), LIM), (dict(inp=None), U), (dict(out=None), U),
+    (dict(heads=-1), U), (dict(heads=32768), LIM), (dict(positions=258), U), (dict(inp=None), U), (dict(out=None), U),
     (dict(positions=None), U), (dict(in_token=-1), U), (dict(in_token=2**22 + 1), LIM),
     (dict(out_head=2**40 + 1), LIM), (dict(out_head=7), U), (dict(out_token=12), U),
     (dict(out_token=8, out_head=8), U),                       # heads and tokens share rows
@@ -109,7 +109,9 @@ def _plan(q=(0, 4), k=None, prefix=None, documents=None, **shape):
     (dict(num_kv_heads=0), U), (dict(num_heads=65538), LIM), (dict(head_dim=0), UNS),
     (dict(head_dim=1025), UNS), (dict(q=(-1, 4)), U), (dict(q=(0, 4, 3)), U),
     (dict(q=(0, 4), k=(2, 1)), U), (dict(q=(0, 2**31)), LIM), (dict(q=(0, 4), k=(0, 2**31)), LIM),
-    (dict(q=(0, 2**30 + 1), num_heads=4, num_kv_heads=2), LIM), (dict(prefix=(-1,)), U)])
+    (dict(q=(0, 2**30 + 1), num_heads=4, num_kv_heads=2), LIM), (dict(prefix=(-1,)), U),
+    (dict(q=(0, 2**31 - 4095), num_heads=1, num_kv_heads=1), LIM),
+    (dict(q=(0, 2**29), num_heads=8, num_kv_heads=8), LIM)])      # groups past a launch
 def test_attention_plans_refuse(change, kind):
     assert _status(lambda: _plan(**change)) == kind
 
