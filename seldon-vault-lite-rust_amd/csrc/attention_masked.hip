@@ -234,8 +234,8 @@ struct TileCopy {
 // ones of head dims that are no whole chunks. Done once a call: splitting floats
 // in every workgroup that reads them was a third of the vector work of the tile
 // kernel (64 documents of 64-512 tokens, 3 heads of 256: 214 us against 181 + 17),
-// and rows of 100 bfloat16 values read one by one took 1296 us for
-// ODD_US (4 x 4096 tokens, 8 heads).
+// and rows of 100 bfloat16 values read one by one took 1296 us against
+// 371 (4 x 4096 tokens, 8 heads).
 template <class T, int P, int D, int KT>
 __global__ __launch_bounds__(256) void masked_planes_kernel(MaskedArgs a) {
     const AttnTiles w = a.tiles[blockIdx.x];

@@ -177,7 +177,7 @@ svl_status fill_positions(svl_position_plan &plan, const svl_segment *segments, 
 // golden ratio, so that each has the short and the long ones of a causal mask;
 // an XCD whose groups are all long would run a second round for a few of them
 // (64 documents of 64-512 tokens: contiguous eighths 191 us, this order
-// ORDER_US). Within an XCD the longest go first, and the short ones end the
+// 161). Within an XCD the longest go first, and the short ones end the
 // launch.
 void order_work(std::vector<AttnWork> &work) {
     constexpr size_t XCDS = 8;
