@@ -1,5 +1,7 @@
 // Attention over packed documents with causal, window and prefix masks, a
 // score cap and a distance bias (svl_masked_attention).
+#include <algorithm>
+
 #include "dev_common.hpp"
 #include "packed.hpp"
 
@@ -289,16 +291,6 @@ __device__ __forceinline__ float other_half_sum(float v) {
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-// tanh(y) / y = 1 + q P(q), q = y^2: a Chebyshev fit of P on [0, 0.56^2], error
-// of tanh 6e-9.
-constexpr float TANH_C0 = -0.33333331f, TANH_C1 = 0.13333082f, TANH_C2 = -0.053903349f,
-                TANH_C3 = 0.021272749f, TANH_C4 = -0.006542542f;
-
-// cap tanh(x / cap) log2(e) from the raw product: to2x = 2 log2(e) scale / cap
-// takes it to the exponent of e^(2 x / cap), capl = cap log2(e).
-// tanh y = 1 - 2 / (e^2y + 1) loses the low bits of a small y (an absolute
-// error of 2^-24): float scores take the series y + y^3 P(y^2) below 0.55
-// (Chebyshev fit of tanh(y) / y, error 4e-8 there).
 // Max / sum over the four 16-lane groups of a wave.
 __device__ __forceinline__ float group_max4(float v) {
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -309,22 +301,26 @@ __device__ __forceinline__ float group_sum4(float v) {
     return other_half_sum(__uint_as_float(a[0]) + __uint_as_float(a[1]));
 }
 
-template <bool EXACT>
+// tanh(y) / y = 1 + q P(q), q = y^2: a Chebyshev fit of P on [0, 0.56^2], error
+// of tanh 6e-9.
+constexpr float TANH_C0 = -0.33333331f, TANH_C1 = 0.13333082f, TANH_C2 = -0.053903349f,
+                TANH_C3 = 0.021272749f, TANH_C4 = -0.006542542f;
+
+// cap tanh(x / cap) log2(e) from the raw product: to2x = 2 log2(e) scale / cap
+// takes it to the exponent of e^(2 x / cap), capl = cap log2(e).
+// tanh y = 1 - 2 / (e^2y + 1) loses the low bits of a small y (an absolute
+// error of 2^-24), which bfloat16 scores do without and float scores take from
+// the series above below 0.55.
 __device__ __forceinline__ float capped(float s, float to2x, float capl) {
     const float z = s * to2x;
     const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(z) + 1.f);
-    float t = __builtin_fmaf(r, -2.f * capl, capl);
-    if constexpr (EXACT) {
-        const float y = z * 0.34657359028f;  // ln 2 / 2
-        const float q = y * y;
-        float p = __builtin_fmaf(q, TANH_C4, TANH_C3);
-        p = __builtin_fmaf(q, p, TANH_C2);
-        p = __builtin_fmaf(q, p, TANH_C1);
-        p = __builtin_fmaf(q, p, TANH_C0);
-        const float small = capl * __builtin_fmaf(y * q, p, y);
-        t = fabsf(y) < 0.55f ? small : t;
-    }
-    return t;
+    const float y = z * 0.34657359028f;  // ln 2 / 2
+    const float q = y * y;
+    float p = __builtin_fmaf(q, TANH_C4, TANH_C3);
+    p = __builtin_fmaf(q, p, TANH_C2);
+    p = __builtin_fmaf(q, p, TANH_C1);
+    p = __builtin_fmaf(q, p, TANH_C0);
+    return fabsf(y) < 0.55f ? capl * __builtin_fmaf(y * q, p, y) : __builtin_fmaf(r, -2.f * capl, capl);
 }
 
 // A workgroup takes WAVES / DS * 32 query vectors of one document and KV head:
@@ -342,6 +338,7 @@ __device__ __forceinline__ float capped(float s, float to2x, float capl) {
 //  * STAGES = 2: a tile's K and V come in under the whole tile before, one
 //    barrier a tile. STAGES = 1, where LDS holds no more: V(t) comes in under
 //    the scores of tile t, K(t + 1) under its softmax and P V; two barriers.
+//    STAGES = 0: K and V in turn in one buffer (512 float dims).
 //  * DS = 2: two waves share 32 queries, each with half of the dims of scores
 //    (summed through LDS) and output, where one wave's registers would leave a
 //    SIMD to a single wave (float rows: three parts of every query; 256 dims
@@ -361,7 +358,7 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
     constexpr int NB = DW / 16, NT = DW / 32, NK = KT / 32, VECTORS = 32 * WAVES / DS;
     // one object a stage, chosen at compile time: the compiler then sees that
     // the DMA into one does not touch the reads of the other
-    __shared__ __bf16 K0[P * KT * D], V0[P * KT * D];
+    __shared__ __bf16 K0[P * KT * D], V0[STAGES > 0 ? P * KT * D : 8];
     __shared__ __bf16 K1[STAGES > 1 ? P * KT * D : 8], V1[STAGES > 1 ? P * KT * D : 8];
     __shared__ f32x4 Sx[DS > 1 ? WAVES * NK * 4 * 64 : 1];  // the waves' parts of the scores
     __shared__ int dirty;  // 1 + the tile whose values hold a non-finite one
@@ -515,7 +512,8 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
             }
         }
     };
-    auto weigh = [&](const __bf16 *Vs, int k0, bool all) {
+    bf16x8 pr[P][NK][2];  // the tile's weights
+    auto weigh = [&](int k0, bool all) {
         if constexpr (DS > 1) {
 #pragma unroll
             for (int kb = 0; kb < NK; ++kb)
@@ -526,24 +524,41 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
                     for (int e = 0; e < 4; ++e) s[kb][r + e] += x[e];
                 }
         }
-        float mul = to_log2;
-        if (CAP || a.slopes || !all) {  // to log2 units first
-            mul = 1.f;
+        // scores in log2 units are s * mul + add
+        float mul = to_log2, add = 0.f;
+        // A capped score is capl - 2 capl r, r = 1 / (e^2y + 1): without a bias
+        // r stays, and the line goes into the exponent's.
+        const bool falling = CAP && P == 1 && !a.slopes;
+        if (falling) {
+            mul = -2.f * capl;
+            add = capl;
+        }
+        if (CAP || a.slopes || !all) {
 #pragma unroll
             for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    s[kb][r] = CAP ? capped<P == 3>(s[kb][r], to2x, capl) : s[kb][r] * to_log2;
+                for (int r = 0; r < 16; ++r) {
+                    if constexpr (CAP && P == 1)
+                        s[kb][r] = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[kb][r] * to2x) + 1.f);
+                    else if constexpr (CAP)
+                        s[kb][r] = capped(s[kb][r], to2x, capl);
+                    else
+                        s[kb][r] *= to_log2;
+                }
+            if (!falling) mul = 1.f;
             if (a.slopes) {
                 const float d0 = (float)(p - k0 - 4 * h);
 #pragma unroll
                 for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
+                    for (int r = 0; r < 16; ++r) {
+                        if constexpr (CAP && P == 1) s[kb][r] = __builtin_fmaf(s[kb][r], -2.f * capl, capl);
                         s[kb][r] = __builtin_fmaf(
                             -slope, fabsf(d0 - (float)(32 * kb + 8 * (r >> 2) + (r & 3))), s[kb][r]);
+                    }
             }
             if (!all) {
+                const float hidden = falling ? INFINITY : -INFINITY;
 #pragma unroll
                 for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
@@ -551,13 +566,12 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
                         // key - lo as an unsigned number is at most hi - lo inside
                         const int key = k0 + 4 * h + 32 * kb + 8 * (r >> 2) + (r & 3);
                         const bool vis = (key < w.prefix) | ((uint32_t)(key - lo) < span);
-                        s[kb][r] = vis ? s[kb][r] : -INFINITY;
+                        s[kb][r] = vis ? s[kb][r] : hidden;
                     }
             }
         }
-        bf16x8 pr[P][NK][2];
         auto exponentials = [&]() {  // the weights, and this lane's sum of them
-            const float base = m_ref == -INFINITY ? 0.f : -m_ref;
+            const float base = add - (m_ref == -INFINITY ? 0.f : m_ref);
             float psum = 0.f;
 #pragma unroll
             for (int kb = 0; kb < NK; ++kb)
@@ -603,12 +617,15 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
             renew = __ballot(!(psum <= MOST_SUM)) != 0;
         }
         if (renew) {
-            float tmax = -INFINITY;
+            float most = -INFINITY, least = INFINITY;
 #pragma unroll
             for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, s[kb][r]);
-            const float m_new = fmaxf(m_ref, other_half_max(tmax) * mul);
+                for (int r = 0; r < 16; ++r) {
+                    most = fmaxf(most, s[kb][r]);
+                    if constexpr (CAP && P == 1) least = fminf(least, s[kb][r]);
+                }
+            const float m_new = fmaxf(m_ref, other_half_max(falling ? __builtin_fmaf(least, mul, add) : most * mul));
             const float alpha = m_ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref - m_new);
             l_run *= alpha;
 #pragma unroll
@@ -617,6 +634,8 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
             psum = exponentials();
         }
         l_run += psum;
+    };
+    auto gather = [&](const __bf16 *Vs) {  // weights times values
 #pragma unroll
         for (int d = 0; d < NT; ++d) {
             const __bf16 *tile = (const __bf16 *)((const char *)Vs + (voff ^ (64 * d)));
@@ -687,7 +706,10 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
             const bool seen = sees(k0);
             if (seen) scores(Ks);
             if constexpr (DS > 1) __syncthreads();  // the other wave's part of the scores
-            if (seen) weigh(Vs, k0, sees_all(k0));
+            if (seen) {
+                weigh(k0, sees_all(k0));
+                gather(Vs);
+            }
         };
         if (w.t0 < w.t1) {
             fetch_k(key_of(w.t0), K0);
@@ -698,6 +720,25 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
             if (redo || t + 1 >= w.t1) break;
             step(t + 1, K1, V1, K0, V0);
             if (redo) break;
+        }
+    } else if constexpr (STAGES == 0) {
+        for (int t = w.t0; t < w.t1; ++t) {
+            const int k0 = key_of(t);
+            asm volatile("" : "+v"(koff), "+v"(voff));
+            fetch_k(k0, K0);
+            kc.commit(K0);
+            __syncthreads();
+            const bool seen = sees(k0);
+            if (seen) scores(K0);
+            __syncthreads();  // no wave reads K any more
+            fetch_v(k0, K0);
+            if (seen) weigh(k0, sees_all(k0));
+            vc.commit(K0);
+            const bool mixed = inspect(K0, t, k0);
+            __syncthreads();
+            if (spoilt(mixed, t)) break;
+            if (seen) gather(K0);
+            __syncthreads();  // nor V
         }
     } else {
         if (w.t0 < w.t1) {
@@ -716,7 +757,10 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
             __syncthreads();  // V has landed; no wave reads K any more
             if (spoilt(mixed, t)) break;
             if (t + 1 < w.t1) fetch_k(key_of(t + 1), K0);
-            if (seen) weigh(V0, k0, sees_all(k0));
+            if (seen) {
+                weigh(k0, sees_all(k0));
+                gather(V0);
+            }
             if (t + 1 < w.t1) kc.commit(K0);
             __syncthreads();  // K has landed; no wave reads V any more
         }
@@ -866,7 +910,7 @@ __global__ __launch_bounds__(256, 2) void masked_few_kernel(MaskedArgs a) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) x = __builtin_fmaf(q[j][e], k[i][e], x);
                 x = group_reduce<16, false>(x);
-                if (a.cap > 0.f) x = capped<true>(x, to2x, capl);
+                if (a.cap > 0.f) x = capped(x, to2x, capl);
                 const int key = k0 + 4 * i;
                 if (a.slopes) x -= slope[j] * fabsf((float)(pos[j] - key));
                 const bool vis = key < w.k_len && (key < w.prefix || (key >= lo[j] && key <= hi[j]));
@@ -1055,8 +1099,8 @@ __global__ __launch_bounds__(256) void masked_join_few_kernel(MaskedArgs a, Mask
 }
 
 // What a batch is run by:
-//  * head dims above 256: a wave a query.
-//  * up to few_vectors float queries of a document and KV head: straight from
+//  * head dims above 512: a wave a query.
+//  * up to eight float queries of a document and KV head (four of 512 dims): straight from
 //    registers (a matrix tile of them took 756 us for 200003 keys, 82 this way);
 //    bfloat16 ones are as fast as the bytes on the matrix cores, 32 to a
 //    workgroup of one wave (4 queries of 128 dims over 2000-8192 keys of 64
@@ -1065,16 +1109,19 @@ __global__ __launch_bounds__(256) void masked_join_few_kernel(MaskedArgs a, Mask
 //    workgroup a CU at 128 dims (prefix mask 1139 -> 1111 us), of 64 for a
 //    fourth at 64 dims (1264 us with tiles of 32, 1137).
 MaskedShape masked_shape(bool bf16, int hd, int64_t most) {
-    if (hd > 256) return {0, 16, ROW_KEYS, 0, 2048, 16};
-    const int dim = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
+    if (hd > 512) return {0, 16, ROW_KEYS, 0, 2048, 16};
+    const int dim = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
     if (bf16) {
         const int planes = hd % 8 ? 1 : 0;
-        if (most <= 32) return {dim, 32, dim == 256 ? 32 : 64, planes, 1280, 1};
-        return {dim, 128, dim == 64 ? 64 : 32, planes, dim == 64 ? 1024 : dim == 128 ? 768 : 512, 8};
+        if (most <= 32) return {dim, 32, dim >= 256 ? 32 : 64, planes, dim == 512 ? 512 : 1280, 1};
+        return {dim, 128, dim == 64 ? 64 : 32, planes, dim == 64 ? 1024 : dim == 128 ? 768 : dim == 256 ? 512 : 256, 8};
     }
-    const int few = dim == 256 ? 4 : 8;
-    if (most <= few) return {dim, most <= 1 ? 1 : most <= 4 ? 4 : 8, few_keys(dim), 0, 512, 1};
-    return {dim, 128, 32, 3, dim == 64 ? 512 : 256, 8};
+    // (a workgroup's registers hold 8, 4 or 2 of them; the rest of 8 are a second group's)
+    if (most <= (dim == 512 ? 4 : 8)) {
+        const int held = dim == 512 ? 2 : dim == 256 ? 4 : 8;
+        return {dim, most <= 1 ? 1 : std::min(held, most <= 4 ? 4 : 8), few_keys(dim), 0, 512, 1};
+    }
+    return {dim, dim == 512 ? 64 : 128, 32, 3, dim == 64 ? 512 : 256, 8};
 }
 
 template <class T, int P, int D, int KT, int WAVES, int DS, int STAGES, TileSource FROM, int MINW,
@@ -1084,7 +1131,7 @@ static hipError_t launch_tiles_capped(const MaskedArgs &a, hipStream_t s) {
     // The sum of rounded weights costs half as much and is what the rounded
     // products are to be divided by, but no lse; it is worth a kernel of its own
     // where vector work bounds it (video 1197 -> 1168 us), not where keys' bytes do.
-    constexpr bool ROUNDED = P == 1 && WAVES > 1 && FROM == FROM_ROWS;
+    constexpr bool ROUNDED = P == 1 && WAVES / DS > 1 && FROM == FROM_ROWS;
     if (ROUNDED && !a.lse)
         hipLaunchKernelGGL((masked_tile_kernel<T, P, D, KT, WAVES, DS, STAGES, FROM, CAP, !ROUNDED, MINW>),
                            grid, block, 0, s, a);
@@ -1116,6 +1163,9 @@ static hipError_t launch_bf16(const MaskedArgs &a, const MaskedShape &shape, hip
             // holds two workgroups)
             return few ? launch_tiles<__bf16, 1, 256, 32, 1, 1, 1, FROM, 1>(a, s)
                        : launch_tiles<__bf16, 1, 256, 32, 4, 1, 2, FROM, 2>(a, s);
+        case 512:
+            return few ? launch_tiles<__bf16, 1, 512, 32, 2, 2, 1, FROM, 1>(a, s)
+                       : launch_tiles<__bf16, 1, 512, 32, 8, 2, 1, FROM, 2>(a, s);
     }
     return hipErrorInvalidValue;
 }
@@ -1146,12 +1196,15 @@ static hipError_t launch_float(const MaskedArgs &a, const MaskedShape &shape, hi
         case 128 * 16 + 8: return launch_few<128, 8>(a, s);
         case 256 * 16 + 1: return launch_few<256, 1>(a, s);
         case 256 * 16 + 4: return launch_few<256, 4>(a, s);
+        case 512 * 16 + 1: return launch_few<512, 1>(a, s);
+        case 512 * 16 + 2: return launch_few<512, 2>(a, s);
         default: return hipErrorInvalidValue;
     }
     switch (shape.dim) {
         case 64: return launch_tiles<float, 3, 64, 32, 4, 1, 2, FROM_PLANES, 2>(a, s);
         case 128: return launch_tiles<float, 3, 128, 32, 8, 2, 2, FROM_PLANES, 2>(a, s);
         case 256: return launch_tiles<float, 3, 256, 32, 8, 2, 1, FROM_PLANES, 2>(a, s);
+        case 512: return launch_tiles<float, 3, 512, 32, 4, 2, 0, FROM_PLANES, 1>(a, s);
     }
     return hipErrorInvalidValue;
 }
@@ -1162,6 +1215,7 @@ static hipError_t launch_planes_of(const MaskedArgs &a, bool bf16, const MaskedS
         case 64: return launch_planes<float, 3, 64, 32>(a, s);
         case 128: return launch_planes<float, 3, 128, 32>(a, s);
         case 256: return launch_planes<float, 3, 256, 32>(a, s);
+        case 512: return launch_planes<float, 3, 512, 32>(a, s);
         default: return hipErrorInvalidValue;
     }
     switch (shape.dim * 64 + shape.keys) {
@@ -1169,6 +1223,7 @@ static hipError_t launch_planes_of(const MaskedArgs &a, bool bf16, const MaskedS
         case 128 * 64 + 64: return launch_planes<__bf16, 1, 128, 64>(a, s);
         case 128 * 64 + 32: return launch_planes<__bf16, 1, 128, 32>(a, s);
         case 256 * 64 + 32: return launch_planes<__bf16, 1, 256, 32>(a, s);
+        case 512 * 64 + 32: return launch_planes<__bf16, 1, 512, 32>(a, s);
     }
     return hipErrorInvalidValue;
 }

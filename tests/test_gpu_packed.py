@@ -225,7 +225,7 @@ def check_attention(seed, ql, kl, nh, nkv, hd, dtype, *, causal=False, window=No
 
 
 TYPES = [F32, BF16]
-HEADS = [(3, 1, 256), (12, 12, 64), (4, 2, 128)]
+HEADS = [(3, 1, 256), (12, 12, 64), (4, 2, 128), (4, 1, 512)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -277,7 +277,8 @@ def test_attention_cap_and_bias(nh, nkv, hd, extra, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("nh,nkv,hd", [(1, 1, 64), (5, 1, 64), (8, 1, 128), (1, 1, 128), (1, 1, 256),
-                                       (9, 1, 128), (40, 1, 64), (6, 3, 100), (3, 1, 250)])
+                                       (9, 1, 128), (40, 1, 64), (6, 3, 100), (3, 1, 250),
+                                       (8, 1, 256), (2, 1, 512), (4, 1, 500), (33, 1, 512)])
 def test_attention_single_queries_by_their_count(nh, nkv, hd, dtype):
     """One query of one to forty heads a KV head, over keys split many and few ways."""
     check_attention(15, [1, 1, 1], [9000, 3, 400], nh, nkv, hd, dtype, causal=True, slopes=nh > 4,
@@ -285,7 +286,8 @@ def test_attention_single_queries_by_their_count(nh, nkv, hd, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("nh,nkv,hd", [(8, 1, 128), (3, 1, 256), (2, 2, 64), (2, 1, 100)])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 1, 128), (3, 1, 256), (2, 2, 64), (2, 1, 100), (4, 1, 512),
+                                       (2, 1, 300)])
 def test_attention_few_long_prompts(nh, nkv, hd, dtype):
     """Few groups of many queries, whose keys are split."""
     check_attention(16, [70, 33], [3500, 2000], nh, nkv, hd, dtype, causal=True,
@@ -315,7 +317,7 @@ def test_attention_reads_nothing_hidden_from_all(ql, mask, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("nh,nkv,hd", HEADS + [(2, 1, 72), (2, 1, 300)])
+@pytest.mark.parametrize("nh,nkv,hd", HEADS + [(2, 1, 72), (2, 1, 300), (1, 1, 700)])
 def test_attention_values_hidden_from_some(nh, nkv, hd, dtype):
     """Under a causal mask a row's own non-finite value reaches it and those after it, and no
     other."""
