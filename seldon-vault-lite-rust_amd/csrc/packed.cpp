@@ -249,11 +249,26 @@ svl_status fill_attention(svl_attention_plan &plan, const int64_t *qo, const int
         const int64_t ql = qo[d + 1] - qo[d], kl = ko[d + 1] - ko[d];
         const int64_t pre = prefix ? std::min(prefix[d], kl) : 0;
         const int64_t shift = kl - ql;
-        const int64_t k_tiles = (kl + KT - 1) / KT, tile0 = (int64_t)tiles.size();
-        if (plan.tiles.planes > 0 && ql > 0)
-            for (int64_t g = 0; g < sh.num_kv_heads; ++g)
-                for (int64_t t = 0; t < k_tiles; ++t)
-                    tiles.push_back({(int32_t)(ko[d] + t * KT), (int32_t)std::min(KT, kl - t * KT), (int32_t)g});
+        // laid out tiles: those that the document's queries see, from the first of them
+        // (a window over a long cache) or of the prefix
+        int64_t from = 0, to = 0;
+        if (plan.tiles.planes > 0 && ql > 0) {
+            int64_t lo = 0, hi = kl - 1;
+            if (sh.causal) hi = std::min(hi, shift + ql - 1);
+            if (sh.window >= 0) {
+                lo = std::max(lo, shift - sh.window);
+                hi = std::min(hi, shift + ql - 1 + sh.window);
+            }
+            to = (pre + KT - 1) / KT;
+            if (hi >= lo) {
+                from = to > 0 ? 0 : lo / KT;
+                to = std::max(to, hi / KT + 1);
+            }
+        }
+        const int64_t tile0 = (int64_t)tiles.size() - from;
+        for (int64_t g = 0; g < sh.num_kv_heads; ++g)
+            for (int64_t t = from; t < to; ++t)
+                tiles.push_back({(int32_t)(ko[d] + t * KT), (int32_t)std::min(KT, kl - t * KT), (int32_t)g});
         for (int64_t g = 0; g < sh.num_kv_heads; ++g)
             for (int64_t v0 = 0; v0 < ql * G; v0 += BV) {
                 // keys that some query of the group sees: the prefix and [lo, hi]
@@ -274,7 +289,7 @@ svl_status fill_attention(svl_attention_plan &plan, const int64_t *qo, const int
                 work.push_back({(int32_t)qo[d], (int32_t)ql, (int32_t)ko[d], (int32_t)kl,
                                 (int32_t)g, (int32_t)v0, (int32_t)pre, (int32_t)pre_tiles,
                                 (int32_t)std::min<int64_t>(first * KT, INT32_MAX), 0,
-                                (int32_t)seen, -1, (int32_t)(tile0 + g * k_tiles)});
+                                (int32_t)seen, -1, (int32_t)(tile0 + g * (to - from))});
             }
     }
     // Groups that leave slots empty, or that are longer than half again the share of

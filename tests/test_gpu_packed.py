@@ -349,6 +349,29 @@ def test_attention_strides(arrange, dtype):
     check_attention(9, [90, 40], [90, 40], 4, 2, 64, dtype, arrange=arrange, causal=True)
 
 
+@pytest.mark.parametrize("dtype,queries", [(BF16, 1), (BF16, 40), (F32, 1), (F32, 40)])
+def test_attention_of_a_cache_past_32_bits(dtype, queries):
+    """Two documents of 4.5 million keys, 2.3 * 10^9 values, seen through a window at their ends:
+    equal to the plain form on those keys alone."""
+    hd, each, window = 256, 4_500_000, 150
+    g = torch.Generator(device=DEV).manual_seed(3)
+    k = torch.empty(2 * each, 1, hd, dtype=dtype, device=DEV).normal_(generator=g)
+    v = torch.empty(2 * each, 1, hd, dtype=dtype, device=DEV).normal_(generator=g)
+    q = torch.empty(2 * queries, 3, hd, dtype=dtype, device=DEV).normal_(generator=g)
+    assert k.numel() > 2**31
+    plan = P.AttentionPlan([0, queries, 2 * queries], [0, each, 2 * each], num_heads=3, num_kv_heads=1,
+                           head_dim=hd, dtype=dtype, causal=True, window=window)
+    assert plan.workspace_bytes < 2**22
+    out = torch.empty_like(q)
+    P.masked_attention(plan, q, k, v, out, 1 / 16)
+    n = queries + window     # the last queries' keys
+    last = torch.cat([torch.arange(e - n, e) for e in (each, 2 * each)])
+    want, _, bound, _ = R.attention(host(q), host(k[last]), host(v[last]),
+                                    [0, queries, 2 * queries], [0, n, 2 * n], causal=True,
+                                    window=window, scale=1 / 16, bf16=dtype == BF16)
+    within(host(out), want, bound)
+
+
 def test_attention_keys_of_one_row():
     """Expanded keys: a token stride of 0."""
     rng = np.random.default_rng(10)
