@@ -767,7 +767,7 @@ __global__ __launch_bounds__(64 * WAVES, MINW) void masked_tile_kernel(MaskedArg
     }
 
     l_run = other_half_sum(l_run);
-    float *part = w.slot < 0 ? nullptr : a.partial + (int64_t)w.slot * (VECTORS * (D + 2));
+    float *part = w.slot < 0 ? nullptr : a.partial + w.slot * masked_slot(VECTORS, D);
     if (redo) {
         for (int i = wave; i < VECTORS && w.v0 + i < nvec; i += WAVES)
             masked_row<T, D / 64>(a, w, w.v0 + i, KT, part ? part + i * D : nullptr,
@@ -969,7 +969,7 @@ __global__ __launch_bounds__(256, 2) void masked_few_kernel(MaskedArgs a) {
         const int vec = w.v0 + j, qi = vec / G, head = w.kvh * G + (vec - qi * G);
         const int64_t qrow = (int64_t)w.q_row + qi;
         T *row = (T *)a.out + qrow * a.o_tok + head * a.o_head;
-        float *part = w.slot < 0 ? nullptr : a.partial + (int64_t)w.slot * (NV * (D + 2));
+        float *part = w.slot < 0 ? nullptr : a.partial + w.slot * masked_slot(NV, D);
 #pragma unroll
         for (int e = 0; e < D / 64; ++e) {
             const int d = lane + 64 * e;
@@ -1007,7 +1007,7 @@ __global__ __launch_bounds__(256) void masked_join_kernel(MaskedArgs a, MaskedSh
     const int local = blockIdx.y, vec = w.v0 + local, dim = blockIdx.z * 32 + 4 * l8;
     if (vec >= w.q_len * G) return;
     const int qi = vec / G, head = w.kvh * G + (vec - qi * G);
-    const int64_t slot = (int64_t)shape.vectors * (shape.dim + 2);  // masked_slot
+    const int64_t slot = masked_slot(shape.vectors, shape.dim);
     const float *part = a.partial + w.slot * slot;
     const float *ml = part + shape.vectors * shape.dim + 2 * local;
     float m[MASKED_MOST_PARTS / 256], l[MASKED_MOST_PARTS / 256], top = -INFINITY;
@@ -1068,7 +1068,7 @@ __global__ __launch_bounds__(256) void masked_join_few_kernel(MaskedArgs a, Mask
     const int G = a.heads / a.kv_heads;
     if (local >= shape.vectors || vec >= w.q_len * G) return;
     const int qi = vec / G, head = w.kvh * G + (vec - qi * G);
-    const int64_t slot = (int64_t)shape.vectors * (shape.dim + 2);  // masked_slot
+    const int64_t slot = masked_slot(shape.vectors, shape.dim);
     const float *part = a.partial + w.slot * slot;
     const float *ml = part + shape.vectors * shape.dim + 2 * local;
     float m[FEW_PARTS], l[FEW_PARTS], top = -INFINITY, sum = 0.f;
@@ -1254,8 +1254,8 @@ hipError_t launch_masked_attention(MaskedArgs a, bool bf16, const MaskedShape &s
                            : launch_bf16<FROM_PIECES>(a, shape, s);
     if (e != hipSuccess || a.n_join == 0) return e;
     const unsigned joins = (unsigned)a.n_join, vectors = (unsigned)a.join_vectors;
-    // (16 parts of one query in the other kernel: 4.5 us, 5.5 here; 4 parts of 128: 3 us here,
-    // 80 there)
+    // (the other kernel's workgroup for each 32 dims of a vector takes 80 us for some 4 parts of 200
+    // groups of 128 queries, which this one joins in a few; a thousand parts want its 32 readers)
     if (a.join_parts <= FEW_PARTS) {
         const unsigned each = 1024u / (unsigned)shape.dim;
         const dim3 grid(joins, (vectors + each - 1) / each), block(256);

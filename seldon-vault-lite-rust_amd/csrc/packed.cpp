@@ -321,7 +321,7 @@ svl_status fill_attention(svl_attention_plan &plan, const int64_t *qo, const int
             if (parts > 1) used += parts;
         }
         work.swap(split);
-        plan.planes_at = used * masked_slot(plan.tiles) * (int64_t)sizeof(float);
+        plan.planes_at = used * masked_slot((int)BV, plan.tiles.dim) * (int64_t)sizeof(float);
     }
     order_work(work);
     plan.n_work = (int32_t)work.size();

@@ -100,8 +100,11 @@ struct MaskedShape {
 };
 // most: query vectors of the batch's largest document and KV head.
 MaskedShape masked_shape(bool bf16, int hd, int64_t most);
-// Floats of a slot of the workspace: outputs, maxima and sums of its vectors.
-inline int64_t masked_slot(const MaskedShape &s) { return (int64_t)s.vectors * (s.dim + 2); }
+// Floats of a slot of the workspace: outputs, maxima and sums of its vectors, in
+// whole 16 bytes.
+constexpr int64_t masked_slot(int vectors, int dim) {
+    return ((int64_t)vectors * (dim + 2) + 3) / 4 * 4;
+}
 // Bytes of a tile of planes: keys and values.
 inline int64_t masked_tile_bytes(const MaskedShape &s) {
     return (int64_t)2 * s.planes * s.keys * s.dim * 2;
