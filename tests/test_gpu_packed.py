@@ -1,6 +1,7 @@
 """The operators on packed documents (axis positions, rotation over several
 axes, masked attention) against plain 64-bit forms, at the sizes, masks,
 strides and types where they can go wrong. packed_ref derives the tolerances."""
+import concurrent.futures
 import math
 
 import numpy as np
@@ -302,6 +303,13 @@ def test_attention_lengths(lengths, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_attention_of_many_documents_and_heads(dtype):
+    check_attention(20, [1] * 3000, [1 + i % 7 for i in range(3000)], 2, 1, 16, dtype)
+    check_attention(21, [1, 2], [300, 70], 128, 1, 64, dtype, causal=True)
+    check_attention(22, [3], [90], 130, 65, 40, dtype, slopes=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_attention_leaves_rows_outside_documents(dtype):
     check_attention(6, [70, 9], [70, 9], 2, 1, 64, dtype, start=3, after=40, poison=True)
 
@@ -447,6 +455,66 @@ def test_attention_bits_do_not_change(dtype):
                 P.masked_attention(plan, qq, k, v, outs[-1], 0.1)
         torch.cuda.synchronize()
         assert all(torch.equal(first, x) for x in outs)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_calls_of_several_threads(dtype):
+    """Threads on streams of their own share a plan: every call's bits are the first one's."""
+    rng = np.random.default_rng(17)
+    o = offsets([500, 3, 210])
+    plans = [P.AttentionPlan(o, num_heads=4, num_kv_heads=2, head_dim=64, dtype=dtype),
+             P.AttentionPlan(np.arange(4), o, num_heads=4, num_kv_heads=2, head_dim=64, dtype=dtype)]
+    q, k, v = (normal(rng, (int(o[-1]), h, 64), dtype)[0] for h in (4, 2, 2))
+    want = [torch.empty_like(q) for _ in plans]
+    for p, w in zip(plans, want):
+        P.masked_attention(p, q, k, v, w, 0.1)
+    torch.cuda.synchronize()
+
+    def work(i):
+        outs = []
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                outs.append(torch.empty_like(q))
+                P.masked_attention(plans[i % 2], q, k, v, outs[-1], 0.1)
+            torch.cuda.current_stream().synchronize()
+        n = plans[i % 2].q_rows
+        return all(torch.equal(x[:n], want[i % 2][:n]) for x in outs)
+
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, range(8)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_plan_let_go_behind_a_call(dtype):
+    """Destroying a plan waits for the work that uses it."""
+    rng = np.random.default_rng(18)
+    n = 6000
+    q, k, v = (normal(rng, (n, h, 128), dtype)[0] for h in (8, 2, 2))
+
+    def call():
+        plan = P.AttentionPlan([0, n], num_heads=8, num_kv_heads=2, head_dim=128, dtype=dtype,
+                               causal=True)
+        out = torch.empty_like(q)
+        for _ in range(3):
+            P.masked_attention(plan, q, k, v, out, 0.1)
+        return out
+
+    first, second = call(), call()
+    torch.cuda.synchronize()
+    assert torch.equal(first, second)
+
+
+def test_attention_refuses_small_and_skew_workspaces():
+    plan = P.AttentionPlan([0, 1], [0, 5000], num_heads=2, num_kv_heads=1, head_dim=64, dtype=F32)
+    q, k = torch.zeros(1, 2, 64, device=DEV), torch.zeros(5000, 1, 64, device=DEV)
+    size = plan.workspace_bytes
+    assert size > 0
+    room = torch.zeros(size + 16, dtype=torch.uint8, device=DEV)
+    for bad in (room[:size - 1], room[1:size + 1], room[:0]):
+        with pytest.raises(svl_amd.SvlError) as e:
+            P.masked_attention(plan, q, k, k, torch.empty_like(q), 1.0, workspace=bad)
+        assert e.value.kind == "Usage"
+    P.masked_attention(plan, q, k, k, torch.empty_like(q), 1.0, workspace=room[:size])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
