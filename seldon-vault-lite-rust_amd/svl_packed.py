@@ -96,12 +96,11 @@ def _rows(name, t, device, dtype, tokens, heads, head_dim):
     """[tokens, heads, head dim], at least `tokens` of them, with a contiguous
     last axis: (data, token stride, head stride). The strides of a single token
     or head are not used."""
-    _on(device, name, t)
     shape = t.shape
     if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim or shape[0] < tokens:
         raise _usage(f"{name} of shape {tuple(shape)}: expected [{tokens}, {heads}, {head_dim}]")
-    if t.dtype != dtype:
-        raise _usage(f"{name} is {t.dtype}, not {dtype}")
+    if t.dtype is not dtype or t.get_device() != device:
+        raise _usage(f"{name} is {t.dtype} on {t.device}, not {dtype} on cuda:{device}")
     token, head, last = t.stride()
     if last != 1 and head_dim > 1 and t.numel():
         raise _usage(f"{name}: the last axis is not contiguous")
@@ -175,16 +174,17 @@ def rope_axes(q, k, positions, inv_freq, pair_axis, layout, out_q, out_k):
         raise _usage("keys and their output come together")
     code, hd = _dtype(dtype), q.shape[2]
     rows, n = b"", 0
-    for name, x, y in (("q", q, out_q), ("k", k, out_k)):
+    for x, y in ((q, out_q), (k, out_k)):
         if x is None:
             continue
-        heads = x.shape[1]
-        data, token, head = _rows(name, x, device, dtype, tokens, heads, hd)
-        out, out_token, out_head = _rows(f"out_{name}", y, device, dtype, tokens, heads, hd)
-        if x.shape[0] != tokens or y.shape[0] != tokens:
-            raise _usage(f"{name} and its output have {x.shape[0]} and {y.shape[0]} tokens, "
-                         f"positions {tokens}")
-        rows += _ROPE_ROWS.pack(data, out, heads, token, head, out_token, out_head)
+        shape = x.shape
+        if shape != y.shape or shape[0] != tokens or len(shape) != 3:
+            raise _usage(f"rows of shape {tuple(shape)} into {tuple(y.shape)}: positions are of "
+                         f"{tokens} tokens")
+        heads = shape[1]
+        data, *strides = _rows("q or k", x, device, dtype, tokens, heads, hd)
+        out, *out_strides = _rows("their output", y, device, dtype, tokens, heads, hd)
+        rows += _ROPE_ROWS.pack(data, out, heads, *strides, *out_strides)
         n += 1
     # bytes pass as pointers that live as long as the call
     call = (rows, n, code, positions.data_ptr(), tokens, axes, hd, freq.tobytes(), axis.tobytes(),
